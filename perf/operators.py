@@ -311,13 +311,17 @@ def _plain_append(s, fp8):
 
 
 def _plain_store_fp8(cache, scales, x, block, offset):
-    """Blocks whose offset 0 is among the new tokens begin anew; the others keep their scale or grow it."""
-    fresh = torch.zeros(cache.shape[0], device="cuda").index_put_((block,), (offset == 0).float(), accumulate=True) > 0
+    """A block whose offset 0 is among the new tokens begins anew; the others keep their scale or grow it, and then the tokens
+    before the new ones are quantised again."""
+    size = cache.shape[1]
+    places = torch.zeros(cache.shape[0], dtype=torch.int64, device="cuda")
+    first = (places + size).scatter_reduce_(0, block, offset, "amin")
     amax = torch.zeros(scales.shape, device="cuda").scatter_reduce_(0, block[:, None].expand(-1, x.shape[1]), x.abs().amax(-1).float(), "amax")
-    touched = torch.zeros(cache.shape[0], device="cuda").index_put_((block,), torch.ones_like(block, dtype=torch.float32), accumulate=True) > 0
-    old = torch.where(fresh[:, None], torch.zeros_like(scales), scales)
-    scale = torch.where(touched[:, None], torch.maximum(old, torch.exp2(_scale_log2(amax).float())), scales)
-    values = cache.view(_E4M3).float() * scales[:, None, :, None] / scale[:, None, :, None]
+    wanted = torch.where((first < size)[:, None], torch.exp2(_scale_log2(amax).float()), torch.zeros_like(scales))
+    scale = torch.where((first == 0)[:, None], wanted, torch.maximum(scales, wanted))
+    before = (torch.arange(size, device="cuda") < first[:, None])[:, :, None, None]
+    values = cache.view(_E4M3).float()
+    values = torch.where(before, values * scales[:, None, :, None] / scale[:, None, :, None], values)
     values[block, offset] = (x / scale[block][..., None]).float()
     cache.copy_(values.clamp(-448, 448).to(_E4M3).view(torch.uint8))
     scales.copy_(scale)
