@@ -252,6 +252,62 @@ INFEROP_API int inferop_paged_attn_decode(void* out, const void* q, const void* 
                               int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, int32_t block_size,
                               int32_t max_blocks_per_seq, float scale, void* stream);
 
+/* Paged attention decode whose scores s = scale q.k are changed before the softmax: softcap tanh(s / softcap) where
+ * softcap > 0, then minus alibi_slopes[head] (seq_len - 1 - t) where there are slopes (fp32 [num_heads], device; NULL:
+ * none).  With neither it is inferop_paged_attn_decode, whose contract holds otherwise.  softcap finite, >= 0.  No
+ * counterpart in the reference. */
+INFEROP_API int inferop_paged_attn_decode_scored(void* out, const void* q, const void* k_cache, const void* v_cache,
+                              const int32_t* block_tables, const int32_t* seq_lens, int32_t dt, int32_t batch,
+                              int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, int32_t block_size,
+                              int32_t max_blocks_per_seq, float scale, float softcap, const float* alibi_slopes,
+                              void* stream);
+
+/* Paged attention decode over 8-bit caches: k_cache / v_cache E4M3 [num_blocks, block_size, num_kv_heads, head_dim]
+ * (16-byte aligned, block_size a multiple of 16), k_scales / v_scales fp32 [num_blocks, num_kv_heads]; a value is its byte
+ * times the scale of its block and head (any finite scale >= 0).  q / out fp16 or bf16.  softcap and alibi_slopes as in
+ * inferop_paged_attn_decode_scored; the rest as in inferop_paged_attn_decode, with its scratch for 16-bit caches.  A
+ * block-table entry outside [0, num_blocks) is a hole: its tokens have no weight; a sequence of holes gives zeros. */
+INFEROP_API int inferop_paged_attn_decode_fp8(void* out, const void* q, const void* k_cache, const void* v_cache,
+                              const void* k_scales, const void* v_scales, const int32_t* block_tables,
+                              const int32_t* seq_lens, int32_t dt, int32_t batch, int32_t num_heads, int32_t num_kv_heads,
+                              int32_t head_dim, int32_t block_size, int32_t num_blocks, int32_t max_blocks_per_seq,
+                              float scale, float softcap, const float* alibi_slopes, void* stream);
+
+/* New tokens into a paged cache, with the rotation on the way (one launch; the reference's caller rotates with rope_neox and
+ * copies rows by itself):
+ *   q [tokens, num_heads, head_dim], k / v [tokens, num_kv_heads, head_dim] in dt, a token's rows contiguous, tokens
+ *   *_stride elements apart (the parts of a fused projection's output); q_out, and k_out where it is not NULL, alike;
+ *   k_cache / v_cache [num_blocks, block_size, num_kv_heads, head_dim] in dt, 16-byte aligned; block_tables int32
+ *   [batch, max_blocks_per_seq]; seq_lens int32 [batch], the lengths WITH the new tokens; cu_seqlens int32 [batch + 1]:
+ *   rows cu_seqlens[b] .. cu_seqlens[b + 1] - 1 are the last tokens of sequence b, or NULL: one token per sequence
+ *   (tokens == batch).
+ * Token i of n has position p = seq_lens[b] - n + i.  q and k are rotated as by inferop_rope_neox (pairs i, i + rotary_dim
+ * / 2; rotary_dim even, 0 .. head_dim; 0: not at all), from angles p base^(-2 i / rotary_dim) yarn_factor that are right at
+ * any position (fp64; inferop_rope_neox multiplies in fp32), and rounded to dt once.  q goes to q_out, k to row p %
+ * block_size of block block_tables[b][p / block_size] of k_cache, and to k_out; v to the same row of v_cache.
+ * Not written: rows in front of cu_seqlens[0] and from cu_seqlens[batch] on and tokens without a position (p < 0); into
+ * the cache, tokens beyond the table or whose entry is outside [0, num_blocks).  q_out may be q and k_out k.  The
+ * sequences of a call must not share blocks that they write to.  head_dim in {64, 128, 256}. */
+INFEROP_API int inferop_rope_append_kv(void* q_out, int64_t q_out_stride, void* k_out, int64_t k_out_stride, void* k_cache,
+                              void* v_cache, const void* q, int64_t q_stride, const void* k, int64_t k_stride,
+                              const void* v, int64_t v_stride, const int32_t* block_tables, const int32_t* seq_lens,
+                              const int32_t* cu_seqlens, int32_t dt, int64_t tokens, int32_t batch, int32_t num_heads,
+                              int32_t num_kv_heads, int32_t head_dim, int32_t rotary_dim, int32_t block_size,
+                              int32_t num_blocks, int32_t max_blocks_per_seq, double base, double yarn_factor, void* stream);
+
+/* The same into 8-bit caches: E4M3 bytes [num_blocks, block_size, num_kv_heads, head_dim], block_size a multiple of 16, and
+ * scales fp32 [num_blocks, num_kv_heads].  What is quantised is the rotated key in fp32 and the value as it is.  The scale of
+ * a block and head is the smallest power of two s with |x| <= 448 s for its finite values, 2^-100 at least.  A token at row 0
+ * begins its block anew; otherwise the scale grows where the new tokens ask for it, and the bytes of the tokens before them
+ * are moved to it (exact but for E4M3's subnormals).  Infinities are stored as +-448 s, NaN as NaN. */
+INFEROP_API int inferop_rope_append_kv_fp8(void* q_out, int64_t q_out_stride, void* k_out, int64_t k_out_stride, void* k_cache,
+                              void* v_cache, void* k_scales, void* v_scales, const void* q, int64_t q_stride, const void* k,
+                              int64_t k_stride, const void* v, int64_t v_stride, const int32_t* block_tables,
+                              const int32_t* seq_lens, const int32_t* cu_seqlens, int32_t dt, int64_t tokens, int32_t batch,
+                              int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, int32_t rotary_dim,
+                              int32_t block_size, int32_t num_blocks, int32_t max_blocks_per_seq, double base,
+                              double yarn_factor, void* stream);
+
 /* SwiGLU (reference include/inferop/ops.h:54-55, kernels/silu_mul.cu:16-28, CPU
  * reference/reference.cpp:55-63): out[t, i] = silu(gate_up[t, i]) * gate_up[t, d + i] for
  * gate_up [tokens, 2d] and out [tokens, d] in dt (0 fp32, 1 fp16, 2 bf16), computed in fp32. */

@@ -8,6 +8,7 @@
 // (kernels/quant.cu:52,72), one "[inferop]" line on stderr for a GEMM contract
 // violation (kernels/gemm/w8a8_block_fp8.cu:167-173).
 #include <cuda_runtime.h>
+#include <math.h>
 #include <stdio.h>
 #include <string.h>
 
@@ -663,10 +664,34 @@ int inferop_rope_neox(void* qkv, const int64_t* positions, int32_t dt, int64_t t
                           static_cast<cudaStream_t>(stream));
 }
 
-int inferop_paged_attn_decode(void* out, const void* q, const void* k_cache, const void* v_cache,
-                              const int32_t* block_tables, const int32_t* seq_lens, int32_t dt, int32_t batch,
-                              int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, int32_t block_size,
-                              int32_t max_blocks_per_seq, float scale, void* stream) {
+// The two appends: fp8 where the scales are given.
+static int kv_append(const KvAppendArgs& a, cudaStream_t s) {
+  if (a.tokens <= 0 || a.batch <= 0 || a.heads <= 0 || a.kv_heads <= 0 || (a.dim != 64 && a.dim != 128 && a.dim != 256) ||
+      a.rotary_dim < 0 || a.rotary_dim > a.dim || (a.rotary_dim & 1) != 0 || a.block_size <= 0 || a.num_blocks <= 0 ||
+      a.max_blocks <= 0 || (!a.cu_seqlens && a.tokens != a.batch) || !(a.base > 0.0 && a.base < INFINITY) ||
+      !(fabs(a.yarn_factor) < INFINITY)) {
+    return INFEROP_ERR_SHAPE;
+  }
+  const int64_t q_row = static_cast<int64_t>(a.heads) * a.dim, kv_row = static_cast<int64_t>(a.kv_heads) * a.dim;
+  if (a.q_stride < q_row || a.k_stride < kv_row || a.v_stride < kv_row || a.q_out_stride < q_row || (a.k_out && a.k_out_stride < kv_row))
+    return INFEROP_ERR_SHAPE;
+  if (a.dt < 0 || a.dt > 2) return INFEROP_ERR_DTYPE;
+  if (a.heads > 65535 || a.kv_heads > 65535 || a.tokens > 0x3FFFFFFF || static_cast<int64_t>(a.max_blocks) * a.block_size > 0x7FFFFF00LL)
+    return INFEROP_ERR_LIMIT;
+  if (!a.q || !a.k || !a.v || !a.q_out || !a.k_cache || !a.v_cache || !a.block_tables || !a.seq_lens) return INFEROP_ERR_POINTER;
+  if ((reinterpret_cast<uintptr_t>(a.k_cache) | reinterpret_cast<uintptr_t>(a.v_cache)) & 15u) return INFEROP_ERR_POINTER;
+  int err;
+  DeviceCtx* ctx = current_ctx(&err);
+  if (!ctx) return err;
+  return launch_kv_append(a, s);
+}
+
+static bool softcap_ok(float cap) { return cap >= 0.0f && cap < INFINITY; }
+
+static int attn_decode(void* out, const void* q, const void* k_cache, const void* v_cache, const Fp8Cache* fp8,
+                       const int32_t* block_tables, const int32_t* seq_lens, int32_t dt, int32_t batch, int32_t num_heads,
+                       int32_t num_kv_heads, int32_t head_dim, int32_t block_size, int32_t max_blocks_per_seq, float scale,
+                       const ScoreMod& mod, void* stream) {
   if (batch <= 0 || num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads != 0 || block_size <= 0 ||
       max_blocks_per_seq <= 0 || (head_dim != 64 && head_dim != 128 && head_dim != 256)) {
     return INFEROP_ERR_SHAPE;
@@ -684,14 +709,14 @@ int inferop_paged_attn_decode(void* out, const void* q, const void* k_cache, con
   // Partial states of a sequence that several CTAs share live in scratch: of this stream or, for a 16-bit
   // call that is being captured, of its graph (a cudaMalloc in the first such call); where none can be had, a
   // 16-bit sequence's heads are one CTA's.
-  if (dt != 0 && paged_attn_on_tensor_cores(batch, num_heads, num_kv_heads, head_dim,
-                                            static_cast<int64_t>(max_blocks_per_seq) * block_size)) {
+  if (fp8 || (dt != 0 && paged_attn_on_tensor_cores(batch, num_heads, num_kv_heads, head_dim,
+                                                    static_cast<int64_t>(max_blocks_per_seq) * block_size))) {
     float* aws = nullptr;
     int* counters = nullptr;
     bool zeroed = false;
     const std::unique_lock<std::mutex> lock = attn_scratch(ctx, s, &aws, &counters, &zeroed);
     return launch_paged_attn_mma(out, q, k_cache, v_cache, block_tables, seq_lens, dt, batch, num_heads, num_kv_heads, head_dim,
-                                 block_size, max_blocks_per_seq, scale, ctx->sm_count, aws, counters, !zeroed, s);
+                                 block_size, max_blocks_per_seq, scale, mod, fp8, ctx->sm_count, aws, counters, !zeroed, s);
   }
   int splits = paged_attn_splits(ctx->sm_count, batch, num_heads, num_kv_heads, block_size, max_blocks_per_seq);
   void *ws = nullptr, *unused = nullptr;
@@ -711,7 +736,62 @@ int inferop_paged_attn_decode(void* out, const void* q, const void* k_cache, con
     }
   }
   return launch_paged_attn_decode(out, q, k_cache, v_cache, block_tables, seq_lens, dt, batch, num_heads, num_kv_heads,
-                                  head_dim, block_size, max_blocks_per_seq, scale, splits, static_cast<float*>(ws), s);
+                                  head_dim, block_size, max_blocks_per_seq, scale, mod, splits, static_cast<float*>(ws), s);
+}
+
+int inferop_rope_append_kv(void* q_out, int64_t q_out_stride, void* k_out, int64_t k_out_stride, void* k_cache, void* v_cache,
+                           const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v, int64_t v_stride,
+                           const int32_t* block_tables, const int32_t* seq_lens, const int32_t* cu_seqlens, int32_t dt,
+                           int64_t tokens, int32_t batch, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                           int32_t rotary_dim, int32_t block_size, int32_t num_blocks, int32_t max_blocks_per_seq, double base,
+                           double yarn_factor, void* stream) {
+  const KvAppendArgs a = {q, k, v, q_out, k_out, k_cache, v_cache, nullptr, nullptr, block_tables, seq_lens, cu_seqlens, q_stride, k_stride,
+                          v_stride, q_out_stride, k_out_stride, tokens, dt, batch, num_heads, num_kv_heads, head_dim, rotary_dim,
+                          block_size, num_blocks, max_blocks_per_seq, base, yarn_factor};
+  return kv_append(a, static_cast<cudaStream_t>(stream));
+}
+
+int inferop_rope_append_kv_fp8(void* q_out, int64_t q_out_stride, void* k_out, int64_t k_out_stride, void* k_cache, void* v_cache,
+                               void* k_scales, void* v_scales, const void* q, int64_t q_stride, const void* k, int64_t k_stride,
+                               const void* v, int64_t v_stride, const int32_t* block_tables, const int32_t* seq_lens,
+                               const int32_t* cu_seqlens, int32_t dt, int64_t tokens, int32_t batch, int32_t num_heads,
+                               int32_t num_kv_heads, int32_t head_dim, int32_t rotary_dim, int32_t block_size, int32_t num_blocks,
+                               int32_t max_blocks_per_seq, double base, double yarn_factor, void* stream) {
+  if (block_size > 0 && block_size % 16 != 0) return INFEROP_ERR_SHAPE;
+  if (!k_scales || !v_scales) return INFEROP_ERR_POINTER;
+  const KvAppendArgs a = {q, k, v, q_out, k_out, k_cache, v_cache, static_cast<float*>(k_scales), static_cast<float*>(v_scales),
+                          block_tables, seq_lens, cu_seqlens, q_stride, k_stride, v_stride, q_out_stride, k_out_stride, tokens, dt, batch,
+                          num_heads, num_kv_heads, head_dim, rotary_dim, block_size, num_blocks, max_blocks_per_seq, base, yarn_factor};
+  return kv_append(a, static_cast<cudaStream_t>(stream));
+}
+
+int inferop_paged_attn_decode(void* out, const void* q, const void* k_cache, const void* v_cache,
+                              const int32_t* block_tables, const int32_t* seq_lens, int32_t dt, int32_t batch,
+                              int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, int32_t block_size,
+                              int32_t max_blocks_per_seq, float scale, void* stream) {
+  return attn_decode(out, q, k_cache, v_cache, nullptr, block_tables, seq_lens, dt, batch, num_heads, num_kv_heads, head_dim, block_size,
+                     max_blocks_per_seq, scale, ScoreMod{}, stream);
+}
+
+int inferop_paged_attn_decode_scored(void* out, const void* q, const void* k_cache, const void* v_cache,
+                                     const int32_t* block_tables, const int32_t* seq_lens, int32_t dt, int32_t batch,
+                                     int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, int32_t block_size,
+                                     int32_t max_blocks_per_seq, float scale, float softcap, const float* alibi_slopes, void* stream) {
+  if (!softcap_ok(softcap)) return INFEROP_ERR_SHAPE;
+  return attn_decode(out, q, k_cache, v_cache, nullptr, block_tables, seq_lens, dt, batch, num_heads, num_kv_heads, head_dim, block_size,
+                     max_blocks_per_seq, scale, ScoreMod{softcap, alibi_slopes}, stream);
+}
+
+int inferop_paged_attn_decode_fp8(void* out, const void* q, const void* k_cache, const void* v_cache, const void* k_scales,
+                                  const void* v_scales, const int32_t* block_tables, const int32_t* seq_lens, int32_t dt, int32_t batch,
+                                  int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, int32_t block_size, int32_t num_blocks,
+                                  int32_t max_blocks_per_seq, float scale, float softcap, const float* alibi_slopes, void* stream) {
+  if (block_size % 16 != 0 || num_blocks <= 0 || !softcap_ok(softcap)) return INFEROP_ERR_SHAPE;
+  if (dt == 0) return INFEROP_ERR_DTYPE;
+  if (!k_scales || !v_scales) return INFEROP_ERR_POINTER;
+  const Fp8Cache fp8 = {static_cast<const float*>(k_scales), static_cast<const float*>(v_scales), num_blocks};
+  return attn_decode(out, q, k_cache, v_cache, &fp8, block_tables, seq_lens, dt, batch, num_heads, num_kv_heads, head_dim, block_size,
+                     max_blocks_per_seq, scale, ScoreMod{softcap, alibi_slopes}, stream);
 }
 
 int inferop_silu_and_mul(void* out, const void* gate_up, int32_t dt, int64_t tokens, int64_t d,

@@ -109,7 +109,9 @@ struct AttnParams {
   const int32_t* seq_lens;
   float* partial;   // [batch][heads][splits][D + 2]: accumulator, running maximum (base 2), denominator
   int num_heads, num_kv_heads, block_size, block_shift, max_blocks_per_seq, splits;   // block_shift: log2(block_size) or -1
-  float scale_log2e;
+  float scale_log2e;     // what q is multiplied by: to base 2 or, capped, to the cap's units
+  float cap_log2e;       // kMod: the cap (0: none), to base 2
+  const float* slopes;   // kMod: a head's loss per token of distance, or null
 };
 
 // element e (0 .. EPL) of a lane's share of a row -> index inside the row
@@ -118,7 +120,8 @@ __device__ __forceinline__ int elem_index(int sub, int e) {
   return ((e / C::EV) * C::LPT + sub) * C::EV + (e % C::EV);
 }
 
-template <typename T, int D, int GT>
+// kMod: scores may be capped and / or fall with distance
+template <typename T, int D, int GT, bool kMod>
 __global__ void __launch_bounds__(kThreads, 4)
 paged_attn_kernel(const AttnParams p) {
   using C = ACfg<T, D>;
@@ -149,6 +152,11 @@ paged_attn_kernel(const AttnParams p) {
     const T* qrow = static_cast<const T*>(p.q) + (static_cast<int64_t>(b) * p.num_heads + head0 + g) * D;
 #pragma unroll
     for (int e = 0; e < C::EPL; ++e) qf[g][e] = to_f32<T>(qrow[elem_index<C>(sub, e)]) * p.scale_log2e;
+  }
+  float slope[kMod ? GT : 1];
+  if constexpr (kMod) {
+#pragma unroll
+    for (int g = 0; g < GT; ++g) slope[g] = p.slopes ? __ldg(p.slopes + head0 + g) * 1.4426950408889634f : 0.0f;
   }
   float m[GT], l[GT], acc[GT][C::EPL];
 #pragma unroll
@@ -263,7 +271,11 @@ paged_attn_kernel(const AttnParams p) {
       constexpr int LF = NV >= C::LPT ? 1 : C::LPT / NV;      // lanes that hold the same total
 #pragma unroll
       for (int v = 0; v < NV; ++v) {
-        const float tot = __shfl_sync(0xFFFFFFFFu, val[v % CF], (v / CF) * LF, C::LPT);
+        float tot = __shfl_sync(0xFFFFFFFFu, val[v % CF], (v / CF) * LF, C::LPT);
+        if constexpr (kMod) {
+          if (p.cap_log2e > 0.0f) tot = p.cap_log2e * tanhf(tot);
+          tot = fmaf(-slope[v / kBatch], static_cast<float>(len - 1 - (tb + v % kBatch * C::NS)), tot);
+        }
         s2[v / kBatch][v % kBatch] = valid[v % kBatch] ? tot : -INFINITY;
       }
     }
@@ -369,7 +381,7 @@ paged_attn_merge_kernel(const AttnParams p) {
   static_cast<T*>(p.out)[head * D + d] = from_f32<T>(mm == -INFINITY ? 0.0f : a / ll);   // (no token at all)
 }
 
-template <typename T, int D, int GT>
+template <typename T, int D, int GT, bool kMod>
 int launch_attn_gt(const AttnParams& p, int batch, cudaStream_t stream) {
   using C = ACfg<T, D>;
   const size_t states = static_cast<size_t>(C::NS) * GT * (D + 2) * sizeof(float);
@@ -379,14 +391,14 @@ int launch_attn_gt(const AttnParams& p, int batch, cudaStream_t stream) {
   int dev = 0;
   cudaGetDevice(&dev);
   if (smem > 48 * 1024 && dev >= 0 && dev < 64 && !attr_done[dev]) {
-    const cudaError_t e = cudaFuncSetAttribute(paged_attn_kernel<T, D, GT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               static_cast<int>(smem));
+    const cudaError_t e = cudaFuncSetAttribute(paged_attn_kernel<T, D, GT, kMod>,
+                                               cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
     if (e != cudaSuccess) return note_cuda_error(e);
     attr_done[dev] = true;
   }
   const int groups = p.num_kv_heads * ((p.num_heads / p.num_kv_heads) / GT);
   const dim3 grid(static_cast<unsigned>(p.splits), static_cast<unsigned>(groups), static_cast<unsigned>(batch));
-  paged_attn_kernel<T, D, GT><<<grid, kThreads, smem, stream>>>(p);
+  paged_attn_kernel<T, D, GT, kMod><<<grid, kThreads, smem, stream>>>(p);
   int rc = check_launch();
   if (rc != INFEROP_OK || p.splits == 1) return rc;
   paged_attn_merge_kernel<T, D><<<dim3(static_cast<unsigned>(p.num_heads), static_cast<unsigned>(batch)), D, 0, stream>>>(p);
@@ -399,23 +411,28 @@ int heads_per_cta(int group) {
   return group % 4 == 0 ? 4 : (group % 2 == 0 ? 2 : 1);
 }
 
-template <typename T, int D>
+template <typename T, int D, bool kMod>
 int launch_attn_d(const AttnParams& p, int batch, cudaStream_t stream) {
   switch (heads_per_cta(p.num_heads / p.num_kv_heads)) {
-    case 4: return launch_attn_gt<T, D, 4>(p, batch, stream);
-    case 2: return launch_attn_gt<T, D, 2>(p, batch, stream);
-    default: return launch_attn_gt<T, D, 1>(p, batch, stream);
+    case 4: return launch_attn_gt<T, D, 4, kMod>(p, batch, stream);
+    case 2: return launch_attn_gt<T, D, 2, kMod>(p, batch, stream);
+    default: return launch_attn_gt<T, D, 1, kMod>(p, batch, stream);
+  }
+}
+
+template <typename T, bool kMod>
+int launch_attn_t(const AttnParams& p, int batch, int head_dim, cudaStream_t stream) {
+  switch (head_dim) {
+    case 64: return launch_attn_d<T, 64, kMod>(p, batch, stream);
+    case 128: return launch_attn_d<T, 128, kMod>(p, batch, stream);
+    case 256: return launch_attn_d<T, 256, kMod>(p, batch, stream);
+    default: return INFEROP_ERR_SHAPE;
   }
 }
 
 template <typename T>
-int launch_attn_t(const AttnParams& p, int batch, int head_dim, cudaStream_t stream) {
-  switch (head_dim) {
-    case 64: return launch_attn_d<T, 64>(p, batch, stream);
-    case 128: return launch_attn_d<T, 128>(p, batch, stream);
-    case 256: return launch_attn_d<T, 256>(p, batch, stream);
-    default: return INFEROP_ERR_SHAPE;
-  }
+int launch_attn_any(const AttnParams& p, bool mod, int batch, int head_dim, cudaStream_t stream) {
+  return mod ? launch_attn_t<T, true>(p, batch, head_dim, stream) : launch_attn_t<T, false>(p, batch, head_dim, stream);
 }
 
 }  // namespace
@@ -443,7 +460,7 @@ size_t paged_attn_workspace_bytes(int splits, int batch, int num_heads, int head
 int launch_paged_attn_decode(void* out, const void* q, const void* k_cache, const void* v_cache,
                              const int32_t* block_tables, const int32_t* seq_lens, int32_t dt, int batch,
                              int num_heads, int num_kv_heads, int head_dim, int block_size, int max_blocks_per_seq,
-                             float scale, int splits, float* workspace, cudaStream_t stream) {
+                             float scale, const ScoreMod& mod, int splits, float* workspace, cudaStream_t stream) {
   AttnParams p;
   p.out = out;
   p.q = q;
@@ -460,11 +477,13 @@ int launch_paged_attn_decode(void* out, const void* q, const void* k_cache, cons
     if ((1 << sh) == block_size) p.block_shift = sh;
   p.max_blocks_per_seq = max_blocks_per_seq;
   p.splits = splits;
-  p.scale_log2e = scale * 1.4426950408889634f;
+  p.scale_log2e = mod.softcap > 0.0f ? scale / mod.softcap : scale * 1.4426950408889634f;
+  p.cap_log2e = mod.softcap * 1.4426950408889634f;
+  p.slopes = mod.slopes;
   switch (dt) {
-    case 0: return launch_attn_t<float>(p, batch, head_dim, stream);
-    case 1: return launch_attn_t<__half>(p, batch, head_dim, stream);
-    case 2: return launch_attn_t<__nv_bfloat16>(p, batch, head_dim, stream);
+    case 0: return launch_attn_any<float>(p, mod.any(), batch, head_dim, stream);
+    case 1: return launch_attn_any<__half>(p, mod.any(), batch, head_dim, stream);
+    case 2: return launch_attn_any<__nv_bfloat16>(p, mod.any(), batch, head_dim, stream);
     default: return INFEROP_ERR_DTYPE;
   }
 }

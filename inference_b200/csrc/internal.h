@@ -20,7 +20,7 @@ int check_launch();
 // Partial states and arrival counters that the CTAs of one paged-attention launch share.
 struct AttnSet {
   static constexpr int kRows = 64;       // launches between two zeroings of the counters
-  static constexpr int kCounters = 320;  // per launch (at least its CTAs)
+  static constexpr int kCounters = 448;  // per launch (at least its CTAs)
   float* ws = nullptr;
   int* counters = nullptr;               // [kRows][kCounters]
   int next_row = kRows;
@@ -175,6 +175,30 @@ int launch_rmsnorm_quant(void* q, void* scales, void* residual, const void* in, 
                          int64_t rows, int64_t cols, float eps, cudaStream_t stream);
 int launch_rope_neox(void* qkv, const int64_t* positions, int32_t dt, int64_t tokens, int heads, int head_dim,
                      int rotary_dim, float base, float yarn, cudaStream_t stream);
+// kv_append.cu : queries and keys rotated, keys and values stored in a paged cache (k_scales null: of the operands' type;
+// else E4M3, block_size a multiple of 16).  Strides are those of a token, in elements; k_out and cu_seqlens may be null.
+struct KvAppendArgs {
+  const void *q, *k, *v;
+  void *q_out, *k_out, *k_cache, *v_cache;
+  float *k_scales, *v_scales;
+  const int32_t *block_tables, *seq_lens, *cu_seqlens;
+  int64_t q_stride, k_stride, v_stride, q_out_stride, k_out_stride, tokens;
+  int32_t dt, batch, heads, kv_heads, dim, rotary_dim, block_size, num_blocks, max_blocks;
+  double base, yarn_factor;
+};
+int launch_kv_append(const KvAppendArgs& a, cudaStream_t stream);
+// What attention does to a score s = scale q.k: softcap tanh(s / softcap) where softcap > 0, then minus slopes[head] times
+// the distance of the two tokens where there are slopes (device, one per query head).
+struct ScoreMod {
+  float softcap = 0.0f;
+  const float* slopes = nullptr;
+  bool any() const { return softcap > 0.0f || slopes != nullptr; }
+};
+// scales of E4M3 caches, [num_blocks][kv_heads]
+struct Fp8Cache {
+  const float *k_scales, *v_scales;
+  int32_t num_blocks;
+};
 // attention.cu : paged attention decode on the CUDA cores.  `splits` token ranges per sequence (paged_attn_splits),
 // `workspace` of paged_attn_workspace_bytes for the partial states when splits > 1 (at most
 // paged_attn_auto_workspace_bytes unless the option attn_splits sets them).
@@ -184,17 +208,17 @@ size_t paged_attn_auto_workspace_bytes(int sm_count);
 int launch_paged_attn_decode(void* out, const void* q, const void* k_cache, const void* v_cache,
                              const int32_t* block_tables, const int32_t* seq_lens, int32_t dt, int batch,
                              int num_heads, int num_kv_heads, int head_dim, int block_size, int max_blocks_per_seq,
-                             float scale, int splits, float* workspace, cudaStream_t stream);
-// attention_mma.cu : on the tensor cores, fp16 (dt 1) / bf16 (dt 2) caches; which calls
-// paged_attn_on_tensor_cores says.  workspace of
+                             float scale, const ScoreMod& mod, int splits, float* workspace, cudaStream_t stream);
+// attention_mma.cu : on the tensor cores, fp16 (dt 1) / bf16 (dt 2) caches, which calls
+// paged_attn_on_tensor_cores says, and E4M3 caches (`fp8`, else nullptr; block_size % 16 == 0), every call.  workspace of
 // paged_attn_mma_workspace_bytes and AttnSet::kCounters zeroed ints of this launch's own; nullptr: every
 // sequence and head group is one CTA's (slower, needs neither).  pdl: programmatic stream serialisation.
 bool paged_attn_on_tensor_cores(int batch, int num_heads, int num_kv_heads, int head_dim, int64_t tokens);
 size_t paged_attn_mma_workspace_bytes();
 int launch_paged_attn_mma(void* out, const void* q, const void* k_cache, const void* v_cache, const int32_t* block_tables,
                           const int32_t* seq_lens, int32_t dt, int batch, int num_heads, int num_kv_heads, int head_dim,
-                          int block_size, int max_blocks_per_seq, float scale, int sm_count, float* workspace, int* counters,
-                          bool pdl, cudaStream_t stream);
+                          int block_size, int max_blocks_per_seq, float scale, const ScoreMod& mod, const Fp8Cache* fp8, int sm_count,
+                          float* workspace, int* counters, bool pdl, cudaStream_t stream);
 int launch_silu_and_mul(void* out, const void* gate_up, int32_t dt, int64_t rows, int64_t d,
                         cudaStream_t stream, int sms);
 int launch_silu_and_mul_quant(void* q, void* scales, const void* gate_up, int32_t dt, int64_t rows,

@@ -431,11 +431,101 @@ def rope_neox(qkv: torch.Tensor, positions: torch.Tensor, rotary_dim: int, base:
     return qkv
 
 
+def _token_rows(t: torch.Tensor, name: str, shape, like: torch.Tensor) -> int:
+    """The stride of a token of t [tokens, heads, dim], whose rows of one token have to be contiguous."""
+    if not t.is_cuda or t.get_device() != like.get_device():
+        raise ValueError(f"{name} must be a CUDA tensor on q's device")
+    if t.dtype != like.dtype or tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} must be {list(shape)} of {like.dtype}, got {list(t.shape)} of {t.dtype}")
+    if t.shape[0] == 0:
+        raise InferopError(_capi.ERR_SHAPE, f"{name} has no tokens")
+    if t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != t.shape[2]):
+        raise ValueError(f"the rows of a token must be contiguous in {name}")
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]
+
+
+def _on_device(like: torch.Tensor, **tensors) -> None:
+    for name, (t, dtype, shape) in tensors.items():
+        _dev_tensor(t, name)
+        if t.get_device() != like.get_device() or t.dtype != dtype or tuple(t.shape) != tuple(shape):
+            raise ValueError(f"{name} must be {dtype} {list(shape)} on q's device, got {t.dtype} {list(t.shape)} on {t.device}")
+
+
+def _append(what, q, k, v, k_cache, v_cache, scales, block_tables, seq_lens, rotary_dim, base, yarn_factor, cu_seqlens, q_out, k_out,
+            stream):
+    if q.dim() != 3 or k.dim() != 3 or k_cache.dim() != 4 or block_tables.dim() != 2 or q.dtype not in _TORCH2CODE:
+        raise ValueError("q must be [tokens, heads, dim] (fp32/fp16/bf16), k and v [tokens, kv_heads, dim], the caches [blocks, "
+                         "block_size, kv_heads, dim] and block_tables [batch, max_blocks]")
+    tokens, heads, dim = q.shape
+    blocks, block_size, kv_heads, _ = k_cache.shape
+    batch, max_blocks = block_tables.shape
+    kv_shape, cache_type = (tokens, kv_heads, dim), q.dtype if scales is None else torch.uint8
+    strides = [_token_rows(q, "q", q.shape, q), _token_rows(k, "k", kv_shape, q), _token_rows(v, "v", kv_shape, q)]
+    _on_device(q, k_cache=(k_cache, cache_type, (blocks, block_size, kv_heads, dim)),
+               v_cache=(v_cache, cache_type, (blocks, block_size, kv_heads, dim)),
+               block_tables=(block_tables, torch.int32, (batch, max_blocks)), seq_lens=(seq_lens, torch.int32, (batch,)))
+    if scales is not None:
+        _on_device(q, k_scales=(scales[0], torch.float32, (blocks, kv_heads)), v_scales=(scales[1], torch.float32, (blocks, kv_heads)))
+    if cu_seqlens is not None:
+        _on_device(q, cu_seqlens=(cu_seqlens, torch.int32, (batch + 1,)))
+    with _on(q):
+        if q_out is None:
+            q_out = torch.empty((tokens, heads, dim), dtype=q.dtype, device=q.device)
+        q_out_stride = _token_rows(q_out, "q_out", q.shape, q)
+        k_out_stride = _token_rows(k_out, "k_out", kv_shape, q) if k_out is not None else 0
+        fn = lib.inferop_rope_append_kv if scales is None else lib.inferop_rope_append_kv_fp8
+        check(fn(q_out.data_ptr(), q_out_stride, k_out.data_ptr() if k_out is not None else None, k_out_stride, k_cache.data_ptr(),
+                 v_cache.data_ptr(), *([] if scales is None else [t.data_ptr() for t in scales]), q.data_ptr(), strides[0],
+                 k.data_ptr(), strides[1], v.data_ptr(), strides[2], block_tables.data_ptr(), seq_lens.data_ptr(),
+                 cu_seqlens.data_ptr() if cu_seqlens is not None else None, _TORCH2CODE[q.dtype], tokens, batch, heads, kv_heads,
+                 dim, int(rotary_dim), block_size, blocks, max_blocks, float(base), float(yarn_factor), _stream_ptr(q, stream)), what)
+    return q_out
+
+
+def rope_append_kv(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                   block_tables: torch.Tensor, seq_lens: torch.Tensor, rotary_dim: int, base: float = 10000.0,
+                   yarn_factor: float = 1.0, cu_seqlens: torch.Tensor | None = None, q_out: torch.Tensor | None = None,
+                   k_out: torch.Tensor | None = None, stream=None) -> torch.Tensor:
+    """New tokens into a paged cache: q and k rotated (NeoX pairs; rotary_dim 0: not), k and v stored; returns the rotated q.
+
+    q [tokens, heads, dim], k / v [tokens, kv_heads, dim]: views of a fused projection's output will do (a token's rows
+    contiguous); caches [blocks, block_size, kv_heads, dim]; seq_lens int32 [batch], the lengths with the new tokens.
+    cu_seqlens int32 [batch + 1]: rows cu_seqlens[b] .. cu_seqlens[b + 1] - 1 are sequence b's last tokens; None: one
+    token per sequence.  k_out: the rotated keys as well (what prefill_attn takes).  q_out may be q, k_out may be k.  Rows that
+    are nobody's are left as they were in q_out and k_out."""
+    return _append("rope_append_kv", q, k, v, k_cache, v_cache, None, block_tables, seq_lens, rotary_dim, base, yarn_factor, cu_seqlens,
+                   q_out, k_out, stream)
+
+
+def rope_append_kv_fp8(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                       k_scales: torch.Tensor, v_scales: torch.Tensor, block_tables: torch.Tensor, seq_lens: torch.Tensor,
+                       rotary_dim: int, base: float = 10000.0, yarn_factor: float = 1.0, cu_seqlens: torch.Tensor | None = None,
+                       q_out: torch.Tensor | None = None, k_out: torch.Tensor | None = None, stream=None) -> torch.Tensor:
+    """rope_append_kv into 8-bit caches: uint8 (E4M3 bytes) with fp32 scales [blocks, kv_heads], block_size a multiple of 16.
+
+    Scales are powers of two.  A token at the first row of a block begins the block anew; later ones let its scale grow where
+    they need it, and the bytes before them move to the new one."""
+    return _append("rope_append_kv_fp8", q, k, v, k_cache, v_cache, (k_scales, v_scales), block_tables, seq_lens, rotary_dim, base,
+                   yarn_factor, cu_seqlens, q_out, k_out, stream)
+
+
+def _slopes_ptr(alibi_slopes, q: torch.Tensor):
+    if alibi_slopes is None:
+        return None
+    _on_device(q, alibi_slopes=(alibi_slopes, torch.float32, (q.shape[1],)))
+    return alibi_slopes.data_ptr()
+
+
 def paged_attn_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor,
-                      seq_lens: torch.Tensor, scale: float, out: torch.Tensor | None = None, stream=None) -> torch.Tensor:
+                      seq_lens: torch.Tensor, scale: float, out: torch.Tensor | None = None, stream=None, softcap: float = 0.0,
+                      alibi_slopes: torch.Tensor | None = None) -> torch.Tensor:
     """q [batch, heads, dim]; k_cache / v_cache [blocks, block_size, kv_heads, dim] (q's dtype); block_tables
-    int32 [batch, max_blocks]; seq_lens int32 [batch] -> [batch, heads, dim]."""
-    if out is None and stream is None and \
+    int32 [batch, max_blocks]; seq_lens int32 [batch] -> [batch, heads, dim].
+
+    softcap > 0: scores are softcap * tanh(score / softcap).  alibi_slopes fp32 [heads]: then minus the head's slope times a
+    token's distance from the last one."""
+    scored = alibi_slopes is not None or softcap != 0.0
+    if not scored and out is None and stream is None and \
             _made(r := fast.paged_attn_decode(q, k_cache, v_cache, block_tables, seq_lens, scale), "paged_attn_decode"):
         return r
     for t, name in ((q, "q"), (k_cache, "k_cache"), (v_cache, "v_cache"), (block_tables, "block_tables"),
@@ -447,15 +537,47 @@ def paged_attn_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
     if block_tables.dtype != torch.int32 or seq_lens.dtype != torch.int32 or block_tables.dim() != 2 or \
             block_tables.shape[0] != q.shape[0] or seq_lens.numel() != q.shape[0]:
         raise ValueError("block_tables must be int32 [batch, max_blocks] and seq_lens int32 [batch]")
+    slopes = _slopes_ptr(alibi_slopes, q)
     batch, heads, dim = q.shape
     _, block_size, kv_heads, _ = k_cache.shape
     with _on(q):
         if out is None:
             out = torch.empty_like(q)
-        check(lib.inferop_paged_attn_decode(out.data_ptr(), q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
-                                            block_tables.data_ptr(), seq_lens.data_ptr(), _TORCH2CODE[q.dtype],
-                                            batch, heads, kv_heads, dim, block_size, block_tables.shape[1],
-                                            float(scale), _stream_ptr(q, stream)), "paged_attn_decode")
+        args = (out.data_ptr(), q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_tables.data_ptr(), seq_lens.data_ptr(),
+                _TORCH2CODE[q.dtype], batch, heads, kv_heads, dim, block_size, block_tables.shape[1], float(scale))
+        if scored:
+            check(lib.inferop_paged_attn_decode_scored(*args, float(softcap), slopes, _stream_ptr(q, stream)), "paged_attn_decode")
+        else:
+            check(lib.inferop_paged_attn_decode(*args, _stream_ptr(q, stream)), "paged_attn_decode")
+    return out
+
+
+def paged_attn_decode_fp8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scales: torch.Tensor,
+                          v_scales: torch.Tensor, block_tables: torch.Tensor, seq_lens: torch.Tensor, scale: float,
+                          softcap: float = 0.0, alibi_slopes: torch.Tensor | None = None, out: torch.Tensor | None = None,
+                          stream=None) -> torch.Tensor:
+    """paged_attn_decode over 8-bit caches (rope_append_kv_fp8): k_cache / v_cache uint8 (E4M3 bytes) [blocks, block_size,
+    kv_heads, dim], block_size a multiple of 16, scales fp32 [blocks, kv_heads]; q fp16 or bf16.  Tokens whose block-table entry
+    is not a block have no weight."""
+    if q.dim() != 3 or q.dtype not in (torch.float16, torch.bfloat16) or k_cache.dim() != 4 or block_tables.dim() != 2:
+        raise ValueError("q must be fp16 or bf16 [batch, heads, dim], the caches [blocks, block_size, kv_heads, dim] and block_tables "
+                         "[batch, max_blocks]")
+    _dev_tensor(q, "q")
+    batch, heads, dim = q.shape
+    blocks, block_size, kv_heads, _ = k_cache.shape
+    cache, scales = (torch.uint8, (blocks, block_size, kv_heads, dim)), (torch.float32, (blocks, kv_heads))
+    _on_device(q, k_cache=(k_cache, *cache), v_cache=(v_cache, *cache), k_scales=(k_scales, *scales), v_scales=(v_scales, *scales),
+               block_tables=(block_tables, torch.int32, (batch, block_tables.shape[1])), seq_lens=(seq_lens, torch.int32, (batch,)))
+    slopes = _slopes_ptr(alibi_slopes, q)
+    with _on(q):
+        if out is None:
+            out = torch.empty_like(q)
+        else:
+            _on_device(q, out=(out, q.dtype, q.shape))
+        check(lib.inferop_paged_attn_decode_fp8(out.data_ptr(), q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scales.data_ptr(),
+                                                v_scales.data_ptr(), block_tables.data_ptr(), seq_lens.data_ptr(), _TORCH2CODE[q.dtype],
+                                                batch, heads, kv_heads, dim, block_size, blocks, block_tables.shape[1], float(scale),
+                                                float(softcap), slopes, _stream_ptr(q, stream)), "paged_attn_decode_fp8")
     return out
 
 
