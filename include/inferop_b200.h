@@ -308,6 +308,21 @@ INFEROP_API int inferop_rope_append_kv_fp8(void* q_out, int64_t q_out_stride, vo
                               int32_t block_size, int32_t num_blocks, int32_t max_blocks_per_seq, double base,
                               double yarn_factor, void* stream);
 
+/* Attention of whole prompts, packed one behind the other (the reference's attention is single-token decode):
+ *   q / out [tokens, num_heads, head_dim], k / v [tokens, num_kv_heads, head_dim] in dt (1 fp16, 2 bf16), a token's rows
+ *   contiguous, tokens *_stride elements apart; cu_seqlens int32 [batch + 1]: prompt b is rows cu_seqlens[b] ..
+ *   cu_seqlens[b + 1] - 1; prefix_lens int32 [batch] or NULL.
+ * Token i of a prompt sees the tokens j < max(i + 1, prefix_lens[b]) of its own: causal without prefixes, everything with one
+ * as long as the prompt.  Scores scale q.k, then softcap and alibi_slopes as in inferop_paged_attn_decode_scored (distance
+ * |i - j|).  Rows in front of cu_seqlens[0] and from cu_seqlens[batch] on are not written.  A value row that is not finite
+ * may reach tokens of its own prompt that do not see it, never another prompt.  Pointers 16-byte aligned, strides
+ * multiples of 8; head_dim in {64, 128, 256}.  The probabilities are rounded to dt for the product with v. */
+INFEROP_API int inferop_prefill_attn(void* out, int64_t out_stride, const void* q, int64_t q_stride, const void* k,
+                              int64_t k_stride, const void* v, int64_t v_stride, const int32_t* cu_seqlens,
+                              const int32_t* prefix_lens, int32_t dt, int64_t tokens, int32_t batch, int32_t num_heads,
+                              int32_t num_kv_heads, int32_t head_dim, float scale, float softcap, const float* alibi_slopes,
+                              void* stream);
+
 /* SwiGLU (reference include/inferop/ops.h:54-55, kernels/silu_mul.cu:16-28, CPU
  * reference/reference.cpp:55-63): out[t, i] = silu(gate_up[t, i]) * gate_up[t, d + i] for
  * gate_up [tokens, 2d] and out [tokens, d] in dt (0 fp32, 1 fp16, 2 bf16), computed in fp32. */

@@ -56,6 +56,8 @@ SIGNATURES = {
                                          _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, C.c_double, C.c_double, _vp]),
     "inferop_rope_append_kv_fp8": (C.c_int, [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _vp,
                                              _i32, _i64, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, C.c_double, C.c_double, _vp]),
+    "inferop_prefill_attn": (C.c_int, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _i32, _i64, _i32, _i32, _i32, _i32,
+                                       C.c_float, C.c_float, _vp, _vp]),
     "inferop_silu_and_mul": (C.c_int, [_vp, _vp, _i32, _i64, _i64, _vp]),
     "inferop_silu_and_mul_quant": (C.c_int, [_vp, _vp, _vp, _i32, _i64, _i64, _i32, _vp]),
     "inferop_moe_max_mtiles": (_i64, [_i64, _i32, _i32]),

@@ -794,6 +794,31 @@ int inferop_paged_attn_decode_fp8(void* out, const void* q, const void* k_cache,
                      max_blocks_per_seq, scale, ScoreMod{softcap, alibi_slopes}, stream);
 }
 
+int inferop_prefill_attn(void* out, int64_t out_stride, const void* q, int64_t q_stride, const void* k, int64_t k_stride,
+                         const void* v, int64_t v_stride, const int32_t* cu_seqlens, const int32_t* prefix_lens, int32_t dt,
+                         int64_t tokens, int32_t batch, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, float scale,
+                         float softcap, const float* alibi_slopes, void* stream) {
+  if (tokens <= 0 || batch <= 0 || num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads != 0 ||
+      (head_dim != 64 && head_dim != 128 && head_dim != 256) || !softcap_ok(softcap)) {
+    return INFEROP_ERR_SHAPE;
+  }
+  const int64_t q_row = static_cast<int64_t>(num_heads) * head_dim, kv_row = static_cast<int64_t>(num_kv_heads) * head_dim;
+  if (out_stride < q_row || q_stride < q_row || k_stride < kv_row || v_stride < kv_row) return INFEROP_ERR_SHAPE;
+  if (dt != 1 && dt != 2) return INFEROP_ERR_DTYPE;
+  if (tokens > 0x7FFFFF00LL || num_heads > 65535) return INFEROP_ERR_LIMIT;
+  if (!out || !q || !k || !v || !cu_seqlens) return INFEROP_ERR_POINTER;
+  if (((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) |
+        reinterpret_cast<uintptr_t>(v)) & 15u) || ((out_stride | q_stride | k_stride | v_stride) & 7)) {
+    return INFEROP_ERR_POINTER;
+  }
+  int err;
+  DeviceCtx* ctx = current_ctx(&err);
+  if (!ctx) return err;
+  const PrefillArgs a = {out, q, k, v, out_stride, q_stride, k_stride, v_stride, tokens, cu_seqlens, prefix_lens, dt, batch, num_heads,
+                         num_kv_heads, head_dim, scale, ScoreMod{softcap, alibi_slopes}};
+  return launch_prefill_attn(ctx, a, static_cast<cudaStream_t>(stream));
+}
+
 int inferop_silu_and_mul(void* out, const void* gate_up, int32_t dt, int64_t tokens, int64_t d,
                          void* stream) {
   if (tokens <= 0 || d <= 0) return INFEROP_ERR_SHAPE;

@@ -1,0 +1,524 @@
+// Attention of whole prompts, packed one behind the other, on the 5th-generation tensor cores (no counterpart in the
+// reference, whose attention is single-token decode).
+//
+//   out[i] = softmax_j(f(scale q_i.k_j)) v_j  over the tokens j < max(i + 1, prefix) of i's own prompt,
+//   f(s) = cap tanh(s / cap) - slope |i - j|
+//
+// One pass over the keys with a running maximum and sum per query row.
+//   * A CTA has two tiles of 128 query rows (two heads of one KV head where the group is even, else 256 rows of a head; one
+//     tile at head size 256), so that the tensor cores work on one while the other's scores are exponentiated.
+//   * S = Q K^T and O += P V are tcgen05.mma with accumulators in tensor memory; P goes back into tensor memory, over the
+//     scores that it came from, and is the A operand from there.  A thread has a row of S: neither maximum nor sum
+//     needs a shuffle.
+//   * K and V blocks come through one ring by TMA.  V lies as it is (tokens outside): operand B with N contiguous.
+//   * O is rescaled only where a row's maximum grew by more than 2^8 since the last time (the exponentials stay below
+//     that), which is rare behind the first blocks; the row's thread does it in tensor memory.
+//   * Rows of a V block behind the prompt's end are set to zero in shared memory: they are another prompt's, and 0 x NaN
+//     would be NaN.  Their scores are masked.
+// P is rounded to the operands' type for the second product: 2^-9 (bf16) or 2^-12 relative per term, of random sign, where
+// the sum is rounded to the same type at the end anyway; row sums are of the unrounded values, in fp32.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include <type_traits>
+
+#include "internal.h"
+#include "ragged.cuh"
+
+namespace ib200 {
+namespace {
+
+constexpr int kTile = 128;                // query rows of a tile: the lanes of tensor memory
+constexpr int kThreads = 320;             // two warpgroups with a row per thread, the issuer of MMAs, the TMA producer
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kRescaleAbove = 8.0f;     // powers of two that a maximum may lag behind
+
+template <int D>
+struct PCfg {
+  static constexpr int kTiles = D == 256 ? 1 : 2;
+  static constexpr int kBlock = D == 256 ? 64 : 128;              // keys of a block
+  static constexpr int kBoxes = D / 64;                           // 128-byte columns of a row
+  static constexpr int kQBytes = kTile * D * 2;                   // of one tile
+  static constexpr int kStageBytes = kBlock * D * 2;              // a K or V block
+  static constexpr int kStages = D == 64 ? 6 : 4;
+  static constexpr int kBarOffset = kTiles * kQBytes + kStages * kStageBytes;
+  static constexpr int kSmemBytes = kBarOffset + 256 + 1024;      // (the base is rounded up to 1024)
+  // tensor memory: two score buffers (one per tile, or of alternate blocks), then the tiles' sums
+  static constexpr int kSCol = 0, kOCol = 2 * kBlock;
+  static_assert(kOCol + kTiles * D <= 512, "tensor memory");
+  static_assert(kSmemBytes <= 232448, "shared memory");
+};
+
+struct PrefillParams {
+  void* out;
+  const int32_t* cu;
+  const int32_t* prefix;   // or null
+  const float* slopes;     // or null
+  int64_t out_stride;
+  int64_t tokens;
+  int batch, heads, kv_heads;
+  int by_heads;            // the two tiles are two heads, not 256 rows of one
+  int groups;              // CTAs side by side over the heads
+  int rows;                // query rows of a head per CTA
+  int slots;               // CTAs over the tokens
+  float scale_log2e;       // what a product is multiplied by: to base 2 or, capped, to the cap's units
+  float cap_log2e;
+  int no_loads;            // test hook: the producer issues no load
+  DeviceStatus* status;
+};
+
+enum : uint32_t {
+  kSiteAProducerEmpty = 0x141,
+  kSiteAProducerEdge = 0x142,
+  kSiteAMmaQ = 0x241,
+  kSiteAMmaFull = 0x242,
+  kSiteAMmaP = 0x243,
+  kSiteASoftmaxS = 0x341,
+  kSiteASoftmaxO = 0x342,
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+template <typename T>
+struct Num;
+template <>
+struct Num<__nv_bfloat16> {
+  static constexpr uint32_t kFormat = 1;
+  static constexpr float kUp = 0.0f;
+  static __device__ __forceinline__ uint32_t pack(float a, float b) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+};
+template <>
+struct Num<__half> {
+  static constexpr uint32_t kFormat = 0;
+  // exponentials are of x + 7: with the maximum's lag they stay below 2^15, and those down to 2^-21 of the maximum's have
+  // all bits of fp16
+  static constexpr float kUp = 7.0f;
+  static __device__ __forceinline__ uint32_t pack(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+};
+
+// A wait of a whole warp: every lane goes on, or none.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile uint32_t* abort_flag, DeviceStatus* status,
+                                          uint32_t site) {
+  return __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity, abort_flag, status, site));
+}
+
+// where a CTA's tile i lies
+struct TileAt {
+  int head, q0, blocks;
+};
+
+template <typename T, int D, bool kMod>
+__global__ void __launch_bounds__(kThreads, 1)
+prefill_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                    const __grid_constant__ CUtensorMap map_v, const PrefillParams p) {
+  using C = PCfg<D>;
+  constexpr int NT = C::kTiles, BN = C::kBlock;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* ring = smem + NT * C::kQBytes;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kBarOffset);
+  uint64_t* q_full = bars;                     // [1]  TMA -> MMA
+  uint64_t* edge = bars + 1;                   // [1]  TMA -> producer: a V block whose tail is set to zero
+  uint64_t* s_full = bars + 2;                 // [2]  MMA -> softmax
+  uint64_t* p_full = bars + 4;                 // [2]  softmax -> MMA (a warp each)
+  uint64_t* o_done = bars + 6;                 // [2]  MMA -> softmax
+  uint64_t* full = bars + 8;                   // [kStages]  TMA -> MMA
+  uint64_t* empty = full + C::kStages;         // [kStages]  MMA -> TMA
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(empty + C::kStages);
+  volatile uint32_t* abort_flag = tmem_slot + 1;
+
+  const int warp = __shfl_sync(0xFFFFFFFFu, static_cast<int>(threadIdx.x >> 5), 0);
+  const int lane = threadIdx.x & 31;
+
+  // ---- this CTA's rows.  Sequence b owns slots from cu[b] / rows + b on (floor(n / rows) + 1 at least, and no sum over the
+  // sequences before); the last rows first: causal ones have the most keys.
+  const int group_at = blockIdx.x % p.groups;
+  const int slot = p.slots - 1 - static_cast<int>(blockIdx.x / p.groups);
+  const int b = last_at_or_below(slot, p.batch, [&](int i) { return static_cast<int64_t>(__ldg(p.cu + i) / p.rows) + i; });
+  if (b < 0) return;
+  const int c0 = __ldg(p.cu + b), c1 = __ldg(p.cu + b + 1);
+  const int n = c1 - c0;
+  const int first_row = (slot - (c0 / p.rows + b)) * p.rows;
+  if (c0 < 0 || c1 > p.tokens || n <= 0 || first_row < 0 || first_row >= n) return;
+  const int prefix = p.prefix ? min(n, max(0, __ldg(p.prefix + b))) : 0;
+  const auto tile_at = [&](int i) {
+    TileAt t;
+    t.head = p.by_heads ? 2 * group_at + i : group_at;
+    t.q0 = first_row + (p.by_heads ? 0 : i * kTile);
+    t.blocks = t.q0 >= n ? 0 : (min(n, max(t.q0 + kTile, prefix)) + BN - 1) / BN;
+    return t;
+  };
+  const TileAt t0 = tile_at(0), t1 = NT == 2 ? tile_at(1) : TileAt{0, 0, 0};
+  const int blocks = max(t0.blocks, t1.blocks);
+  const int kv_col = t0.head / (p.heads / p.kv_heads) * D;
+
+  if (threadIdx.x == 0) {
+    mbar_init(q_full, 1);
+    mbar_init(edge, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 4);
+      mbar_init(&o_done[i], 1);
+    }
+    for (int s = 0; s < C::kStages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    *abort_flag = 0u;
+    mbar_init_fence();
+    tma_prefetch_desc(&map_q);
+    tma_prefetch_desc(&map_k);
+    tma_prefetch_desc(&map_v);
+  }
+  if (warp == 8) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, *tmem_slot, 0);
+
+  if (warp == 9) {
+    // ------------------------------ TMA producer ------------------------
+    bool ok = true;
+    if (!p.no_loads) {
+      if (lane == 0) {
+        mbar_arrive_expect_tx(q_full, NT * C::kQBytes);   // (a tile without rows is loaded too: nothing of it is stored)
+        for (int i = 0; i < NT; ++i) {
+          const TileAt t = i == 0 ? t0 : t1;
+          for (int x = 0; x < C::kBoxes; ++x)
+            tma_load_2d(smem + i * C::kQBytes + x * (kTile * 128), &map_q, q_full, t.head * D + x * 64, c0 + t.q0);
+        }
+      }
+      int stage = 0;
+      uint32_t phase = 0;
+      for (int it = 0; it < 2 * blocks; ++it) {           // K 0, V 0, K 1, V 1, ...
+        const int j = it >> 1;
+        const bool is_v = (it & 1) != 0;
+        if (!warp_wait(&empty[stage], phase ^ 1u, abort_flag, p.status, kSiteAProducerEmpty)) {
+          ok = false;
+          break;
+        }
+        uint8_t* dst = ring + stage * C::kStageBytes;
+        const bool tail = is_v && (j + 1) * BN > n;        // (once, in the last block of the prompt)
+        uint64_t* bar = tail ? edge : &full[stage];
+        if (lane == 0) {
+          mbar_arrive_expect_tx(bar, C::kStageBytes);
+          for (int x = 0; x < C::kBoxes; ++x)
+            tma_load_2d(dst + x * (BN * 128), is_v ? &map_v : &map_k, bar, kv_col + x * 64, c0 + j * BN);
+        }
+        __syncwarp();
+        if (tail) {
+          if (!warp_wait(edge, 0u, abort_flag, p.status, kSiteAProducerEdge)) {
+            ok = false;
+            break;
+          }
+          const int r0 = n - j * BN;                       // the swizzle moves 16-byte pieces inside a row only
+          for (int x = 0; x < C::kBoxes; ++x)
+            for (int i = r0 * 8 + lane; i < BN * 8; i += 32)
+              reinterpret_cast<uint4*>(dst + x * (BN * 128))[i] = make_uint4(0u, 0u, 0u, 0u);
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&full[stage]);
+        }
+        if (++stage == C::kStages) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+    }
+    if (!ok) {
+      // copies that this warp started may still be on their way: give them time to land before the CTA ends
+      const long long w0 = clock64();
+      while (clock64() - w0 < (1LL << 22)) {
+      }
+    }
+  } else if (warp == 8) {
+    // ------------------------------ MMA issuer --------------------------
+    constexpr uint32_t idesc_s = umma_idesc_16bit_f32(Num<T>::kFormat, kTile, BN, false);
+    constexpr uint32_t idesc_o = umma_idesc_16bit_f32(Num<T>::kFormat, kTile, D, true);
+    const uint32_t q_addr = smem_u32(smem), ring_addr = smem_u32(ring);
+    // K block j is element 2 j of the ring's sequence, V block j element 2 j + 1
+    auto stage_of = [&](int it) { return it % C::kStages; };
+    auto wait_full = [&](int it) {
+      return warp_wait(&full[stage_of(it)], (it / C::kStages) & 1, abort_flag, p.status, kSiteAMmaFull);
+    };
+    auto scores = [&](int i, int j) {       // S = Q_i K_j^T
+      const uint32_t d = tmem + C::kSCol + (NT == 2 ? i : j & 1) * BN;
+      const uint32_t k = ring_addr + stage_of(2 * j) * C::kStageBytes, q = q_addr + i * C::kQBytes;
+      if (elect_one()) {
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          const uint32_t in_box = (kk % 4) * 32;
+          umma_16bit_ss(d, umma_desc_k_sw128(q + (kk / 4) * (kTile * 128) + in_box), umma_desc_k_sw128(k + (kk / 4) * (BN * 128) + in_box),
+                        idesc_s, kk > 0 ? 1u : 0u);
+        }
+        umma_commit(&s_full[NT == 2 ? i : j & 1]);
+      }
+      __syncwarp();
+    };
+    auto sums = [&](int i, int j) {         // O_i += P V_j
+      const uint32_t a = tmem + C::kSCol + (NT == 2 ? i : j & 1) * BN;
+      const uint32_t v = ring_addr + stage_of(2 * j + 1) * C::kStageBytes;
+      if (elect_one()) {
+#pragma unroll
+        for (int kk = 0; kk < BN / 16; ++kk)
+          umma_16bit_ts(tmem + C::kOCol + i * D, a + kk * 8, umma_desc_mn_sw128(v + kk * 2048, BN * 128), idesc_o, j > 0 || kk > 0 ? 1u : 0u);
+        umma_commit(&o_done[i]);
+      }
+      __syncwarp();
+    };
+    auto release = [&](int it) {
+      if (elect_one()) umma_commit(&empty[stage_of(it)]);
+      __syncwarp();
+    };
+    auto wait_p = [&](int i, int j) {
+      return warp_wait(&p_full[NT == 2 ? i : j & 1], (NT == 2 ? j : j >> 1) & 1, abort_flag, p.status, kSiteAMmaP);
+    };
+    const int tile_blocks[2] = {t0.blocks, t1.blocks};
+    bool ok = warp_wait(q_full, 0u, abort_flag, p.status, kSiteAMmaQ) && wait_full(0);
+    if (ok) {
+      tc_fence_after_sync();
+#pragma unroll
+      for (int i = 0; i < NT; ++i)
+        if (tile_blocks[i] > 0) scores(i, 0);
+      release(0);
+    }
+    for (int j = 0; ok && j < blocks; ++j) {
+      if (NT == 1 && j + 1 < blocks) {
+        ok = wait_full(2 * j + 2);
+        if (!ok) break;
+        tc_fence_after_sync();
+        scores(0, j + 1);
+        release(2 * j + 2);
+      }
+      ok = wait_full(2 * j + 1);
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+        if (!ok) break;
+        if (j < tile_blocks[i]) {
+          ok = wait_p(i, j);
+          if (!ok) break;
+          tc_fence_after_sync();
+          sums(i, j);
+        }
+        if (i == NT - 1) release(2 * j + 1);
+        if (NT == 2 && j + 1 < blocks) {
+          if (i == 0) ok = wait_full(2 * j + 2);
+          if (!ok) break;
+          tc_fence_after_sync();
+          if (j + 1 < tile_blocks[i]) scores(i, j + 1);
+          if (i == 1) release(2 * j + 2);
+        }
+      }
+    }
+  } else if (warp < 4 * NT) {
+    // ------------------------------ softmax: a thread per row -----------
+    const int i = warp >> 2;
+    const TileAt t = i == 0 ? t0 : t1;
+    const int pos = t.q0 + (warp & 3) * 32 + lane;
+    const int lim = min(n, max(pos + 1, prefix));          // keys from here on are masked (rows behind the prompt: any)
+    const int lim_warp = __shfl_sync(0xFFFFFFFFu, lim, 0);
+    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t o_at = tmem + lanes + C::kOCol + i * D;
+    const float slope = kMod && p.slopes ? __ldg(p.slopes + t.head) * kLog2e : 0.0f;
+    float m = -INFINITY, l = 0.0f;                         // m: what the row's exponentials are relative to, base 2
+    bool ok = true;
+    for (int j = 0; j < t.blocks; ++j) {
+      const int buf = NT == 2 ? i : j & 1;
+      const uint32_t s_at = tmem + lanes + C::kSCol + buf * BN;
+      ok = warp_wait(&s_full[buf], (NT == 2 ? j : j >> 1) & 1, abort_flag, p.status, kSiteASoftmaxS);
+      if (!ok) break;
+      tc_fence_after_sync();
+      uint32_t s[BN / 32][32];
+#pragma unroll
+      for (int c = 0; c < BN / 32; ++c) tmem_ld_32x32(s_at + c * 32, s[c]);
+      tmem_ld_wait();
+#pragma unroll
+      for (int c = 0; c < BN / 32; ++c) pin32(s[c]);
+      if constexpr (kMod) {
+#pragma unroll
+        for (int c = 0; c < BN / 32; ++c) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            float x = __uint_as_float(s[c][e]) * p.scale_log2e;
+            if (p.cap_log2e > 0.0f) {
+              // tanh(x) = 1 - 2 / (1 + e^2x): off by some 2^-22, which the cap multiplies
+              float r;
+              asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + ex2(x * (2.0f * kLog2e))));
+              x = p.cap_log2e * fmaf(-2.0f, r, 1.0f);
+            }
+            s[c][e] = __float_as_uint(fmaf(-slope, fabsf(static_cast<float>(pos - (j * BN + c * 32 + e))), x));
+          }
+        }
+      }
+      if ((j + 1) * BN > lim_warp) {
+#pragma unroll
+        for (int c = 0; c < BN / 32; ++c) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            if (j * BN + c * 32 + e >= lim) s[c][e] = 0xFF800000u;   // -inf
+        }
+      }
+      const float f = kMod ? 1.0f : p.scale_log2e;
+      float mx[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) mx[e] = __uint_as_float(s[0][e]);
+#pragma unroll
+      for (int c = 0; c < BN / 32; ++c) {
+#pragma unroll
+        for (int e = c == 0 ? 4 : 0; e < 32; ++e) mx[e & 3] = fmaxf(mx[e & 3], __uint_as_float(s[c][e]));
+      }
+      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * f;
+      // (rows behind the prompt have no say: a prompt's bits do not depend on its neighbours)
+      if (__any_sync(0xFFFFFFFFu, pos < n && (top > m + kRescaleAbove || m == -INFINITY))) {
+        const float m_new = fmaxf(m, top);
+        const float alpha = m_new == -INFINITY ? 1.0f : ex2(m - m_new);   // (every score so far -inf: no weight, not NaN)
+        l *= alpha;
+        m = m_new;
+        if (j > 0) {
+          // the product before is the last one on these sums until this warp's next arrival
+          ok = warp_wait(&o_done[i], (j - 1) & 1, abort_flag, p.status, kSiteASoftmaxO);
+          if (!ok) break;
+          tc_fence_after_sync();
+#pragma unroll 1
+          for (int c = 0; c < D; c += 32) {
+            uint32_t o[32];
+            tmem_ld_32x32(o_at + c, o);
+            tmem_ld_wait();
+            pin32(o);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+            tmem_st_32x32(o_at + c, o);
+          }
+        }
+      }
+      const float ref = (m == -INFINITY ? 0.0f : m) - Num<T>::kUp;
+      const float2 f2 = make_float2(f, f), ref2 = make_float2(-ref, -ref);
+      float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+#pragma unroll
+      for (int c = 0; c < BN / 32; ++c) {
+        uint32_t w[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          float2 x = make_float2(__uint_as_float(s[c][2 * e]), __uint_as_float(s[c][2 * e + 1]));
+          x = kMod ? __fadd2_rn(x, ref2) : __ffma2_rn(x, f2, ref2);
+          x.x = ex2(x.x);
+          x.y = ex2(x.y);
+          sum[e & 1] = __fadd2_rn(sum[e & 1], x);
+          w[e] = Num<T>::pack(x.x, x.y);
+        }
+        tmem_st_32x16(s_at + c * 16, w);
+      }
+      l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+      tmem_st_wait();
+      tc_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&p_full[buf]);
+    }
+    // ---- the row's sums / l
+    if (t.blocks > 0 && ok) {
+      if (warp_wait(&o_done[i], (t.blocks - 1) & 1, abort_flag, p.status, kSiteASoftmaxO)) {
+        tc_fence_after_sync();
+        const float inv = 1.0f / l;
+        T* dst = static_cast<T*>(p.out) + (static_cast<int64_t>(c0) + pos) * p.out_stride + static_cast<int64_t>(t.head) * D;
+#pragma unroll 1
+        for (int c = 0; c < D; c += 32) {
+          uint32_t o[32];
+          tmem_ld_32x32(o_at + c, o);
+          tmem_ld_wait();
+          pin32(o);
+          if (pos < n) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 8) {
+              uint4 w;
+              w.x = Num<T>::pack(__uint_as_float(o[e]) * inv, __uint_as_float(o[e + 1]) * inv);
+              w.y = Num<T>::pack(__uint_as_float(o[e + 2]) * inv, __uint_as_float(o[e + 3]) * inv);
+              w.z = Num<T>::pack(__uint_as_float(o[e + 4]) * inv, __uint_as_float(o[e + 5]) * inv);
+              w.w = Num<T>::pack(__uint_as_float(o[e + 6]) * inv, __uint_as_float(o[e + 7]) * inv);
+              *reinterpret_cast<uint4*>(dst + c + e) = w;
+            }
+          }
+        }
+      }
+    }
+  }
+  __syncwarp();
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  if (warp == 8) tmem_dealloc(tmem, 512);
+}
+
+template <typename T, int D, bool kMod>
+int launch_d(const PrefillArgs& a, PrefillParams p, cudaStream_t stream) {
+  using C = PCfg<D>;
+  const auto kernel = prefill_attn_kernel<T, D, kMod>;
+  static bool attr_done[64] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev >= 0 && dev < 64 && !attr_done[dev]) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes);
+    if (e != cudaSuccess) return note_cuda_error(e);
+    attr_done[dev] = true;
+  }
+  p.by_heads = C::kTiles == 2 && a.heads / a.kv_heads % 2 == 0 ? 1 : 0;
+  p.groups = p.by_heads ? a.heads / 2 : a.heads;
+  p.rows = p.by_heads ? kTile : C::kTiles * kTile;
+  const int64_t slots = a.tokens / p.rows + a.batch;
+  if (slots * p.groups > 0x7FFFFFFF) return INFEROP_ERR_LIMIT;
+  p.slots = static_cast<int>(slots);
+  CUtensorMap mq, mk, mv;
+  int rc = make_tensor_map_2d(&mq, a.q, 2, a.tokens, static_cast<uint64_t>(a.heads) * D, a.q_stride * 2, kTile, 64, true);
+  if (rc == INFEROP_OK) rc = make_tensor_map_2d(&mk, a.k, 2, a.tokens, static_cast<uint64_t>(a.kv_heads) * D, a.k_stride * 2, C::kBlock, 64, true);
+  if (rc == INFEROP_OK) rc = make_tensor_map_2d(&mv, a.v, 2, a.tokens, static_cast<uint64_t>(a.kv_heads) * D, a.v_stride * 2, C::kBlock, 64, true);
+  if (rc != INFEROP_OK) return rc;
+  kernel<<<static_cast<unsigned>(slots * p.groups), kThreads, C::kSmemBytes, stream>>>(mq, mk, mv, p);
+  return check_launch();
+}
+
+template <typename T, bool kMod>
+int launch_t(const PrefillArgs& a, const PrefillParams& p, cudaStream_t stream) {
+  switch (a.dim) {
+    case 64: return launch_d<T, 64, kMod>(a, p, stream);
+    case 128: return launch_d<T, 128, kMod>(a, p, stream);
+    case 256: return launch_d<T, 256, kMod>(a, p, stream);
+    default: return INFEROP_ERR_SHAPE;
+  }
+}
+
+}  // namespace
+
+int launch_prefill_attn(DeviceCtx* ctx, const PrefillArgs& a, cudaStream_t stream) {
+  PrefillParams p = {};
+  p.out = a.out;
+  p.cu = a.cu_seqlens;
+  p.prefix = a.prefix_lens;
+  p.slopes = a.mod.slopes;
+  p.out_stride = a.out_stride;
+  p.tokens = a.tokens;
+  p.batch = a.batch, p.heads = a.heads, p.kv_heads = a.kv_heads;
+  p.scale_log2e = a.mod.softcap > 0.0f ? a.scale / a.mod.softcap : a.scale * kLog2e;
+  p.cap_log2e = a.mod.softcap * kLog2e;
+  p.no_loads = options().debug_no_loads;
+  p.status = ctx->status;
+  // (the plain form takes the maximum of the products and scales it, so it needs a positive scale)
+  const bool mod = a.mod.any() || !(a.scale > 0.0f);
+  if (a.dt == 1) return mod ? launch_t<__half, true>(a, p, stream) : launch_t<__half, false>(a, p, stream);
+  return mod ? launch_t<__nv_bfloat16, true>(a, p, stream) : launch_t<__nv_bfloat16, false>(a, p, stream);
+}
+
+}  // namespace ib200

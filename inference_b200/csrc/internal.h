@@ -219,6 +219,17 @@ int launch_paged_attn_mma(void* out, const void* q, const void* k_cache, const v
                           const int32_t* seq_lens, int32_t dt, int batch, int num_heads, int num_kv_heads, int head_dim,
                           int block_size, int max_blocks_per_seq, float scale, const ScoreMod& mod, const Fp8Cache* fp8, int sm_count,
                           float* workspace, int* counters, bool pdl, cudaStream_t stream);
+// attention_prefill.cu : attention of packed prompts, fp16 (dt 1) / bf16 (dt 2).  Strides are those of a token, in elements.
+struct PrefillArgs {
+  void* out;
+  const void *q, *k, *v;
+  int64_t out_stride, q_stride, k_stride, v_stride, tokens;
+  const int32_t *cu_seqlens, *prefix_lens;   // prefix_lens may be null
+  int32_t dt, batch, heads, kv_heads, dim;
+  float scale;
+  ScoreMod mod;
+};
+int launch_prefill_attn(DeviceCtx* ctx, const PrefillArgs& a, cudaStream_t stream);
 int launch_silu_and_mul(void* out, const void* gate_up, int32_t dt, int64_t rows, int64_t d,
                         cudaStream_t stream, int sms);
 int launch_silu_and_mul_quant(void* q, void* scales, const void* gate_up, int32_t dt, int64_t rows,

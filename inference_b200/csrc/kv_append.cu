@@ -25,6 +25,7 @@
 #include <stdint.h>
 
 #include "internal.h"
+#include "ragged.cuh"
 
 namespace ib200 {
 namespace {
@@ -77,24 +78,6 @@ template <int V>
 struct alignas(V) Bytes {
   uint8_t e[V];
 };
-
-// The sequence that holds key t of the nondecreasing list key(0) <= key(1) <= ..., -1 before the first; the whole warp.
-// 32 places per step.  (What a list in another order gives is some index in range.)
-template <typename F>
-__device__ __forceinline__ int last_at_or_below(int64_t t, int n, F key) {
-  const int lane = threadIdx.x & 31;
-  int lo = 0, count = n;
-  while (true) {
-    const int step = (count + 31) / 32;
-    const int at = lo + lane * step;
-    const bool in = lane * step < count && key(at) <= t;
-    const int c = __popc(__ballot_sync(0xFFFFFFFFu, in));
-    if (c == 0) return -1;
-    lo += (c - 1) * step;
-    if (step == 1) return lo;
-    count = min(step, count - (c - 1) * step);
-  }
-}
 
 // where a token lies: its position (-1: nobody's token) and its cache row (-1: none)
 struct Place {

@@ -581,6 +581,36 @@ def paged_attn_decode_fp8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch
     return out
 
 
+def prefill_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor, scale: float, softcap: float = 0.0,
+                 alibi_slopes: torch.Tensor | None = None, prefix_lens: torch.Tensor | None = None,
+                 out: torch.Tensor | None = None, stream=None) -> torch.Tensor:
+    """Attention of whole prompts, packed one behind the other: q [tokens, heads, dim], k / v [tokens, kv_heads, dim] (fp16 or
+    bf16; views of a fused projection's output will do) -> [tokens, heads, dim].
+
+    cu_seqlens int32 [batch + 1]: prompt b is rows cu_seqlens[b] .. cu_seqlens[b + 1] - 1; other rows of `out` are left as they
+    were.  Causal; prefix_lens int32 [batch]: every token of a prompt sees its first so many.  softcap and alibi_slopes as in
+    paged_attn_decode."""
+    if q.dim() != 3 or k.dim() != 3 or cu_seqlens.dim() != 1 or q.dtype not in (torch.float16, torch.bfloat16):
+        raise ValueError("q must be fp16 or bf16 [tokens, heads, dim], k and v [tokens, kv_heads, dim], cu_seqlens [batch + 1]")
+    tokens, heads, dim = q.shape
+    kv_heads, batch = k.shape[1], cu_seqlens.shape[0] - 1
+    kv_shape = (tokens, kv_heads, dim)
+    strides = [_token_rows(q, "q", q.shape, q), _token_rows(k, "k", kv_shape, q), _token_rows(v, "v", kv_shape, q)]
+    _on_device(q, cu_seqlens=(cu_seqlens, torch.int32, (batch + 1,)))
+    if prefix_lens is not None:
+        _on_device(q, prefix_lens=(prefix_lens, torch.int32, (batch,)))
+    slopes = _slopes_ptr(alibi_slopes, q)
+    with _on(q):
+        if out is None:
+            out = torch.empty((tokens, heads, dim), dtype=q.dtype, device=q.device)
+        check(lib.inferop_prefill_attn(out.data_ptr(), _token_rows(out, "out", q.shape, q), q.data_ptr(), strides[0], k.data_ptr(),
+                                       strides[1], v.data_ptr(), strides[2], cu_seqlens.data_ptr(),
+                                       prefix_lens.data_ptr() if prefix_lens is not None else None, _TORCH2CODE[q.dtype], tokens, batch,
+                                       heads, kv_heads, dim, float(scale), float(softcap), slopes, _stream_ptr(q, stream)),
+              "prefill_attn")
+    return out
+
+
 def silu_and_mul(gate_up: torch.Tensor, out: torch.Tensor | None = None, stream=None) -> torch.Tensor:
     """out[t, i] = silu(gate_up[t, i]) * gate_up[t, d + i] (reference include/inferop/ops.h:54-55)."""
     _dev_tensor(gate_up, "gate_up")

@@ -50,11 +50,11 @@ def attention(q, k, v, scale, cap=0.0, slopes=None, seen=None, pos=None):
     """q [n, heads, dim] over k / v [m, kv_heads, dim]; seen [n, m] or None; pos: position of each query (default: the last n)."""
     n, heads, dim = q.shape
     m, kv, _ = k.shape
-    out = torch.zeros(n, heads, dim, dtype=torch.float64)
+    out = torch.zeros(n, heads, dim, dtype=torch.float64, device=q.device)
     if m == 0:
         return out
-    pos = torch.arange(m - n, m) if pos is None else pos
-    far = (pos[:, None] - torch.arange(m)[None, :]).abs().double()
+    pos = torch.arange(m - n, m, device=q.device) if pos is None else pos
+    far = (pos[:, None] - torch.arange(m, device=q.device)[None, :]).abs().double()
     for h in range(heads):
         g = h // (heads // kv)
         s = q[:, h].double() @ k[:, g].double().T * scale
