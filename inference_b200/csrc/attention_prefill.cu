@@ -32,7 +32,9 @@ namespace ib200 {
 namespace {
 
 constexpr int kTile = 128;                // query rows of a tile: the lanes of tensor memory
-constexpr int kThreads = 320;             // two warpgroups with a row per thread, the issuer of MMAs, the TMA producer
+// two warpgroups with a row per thread; the issuer of MMAs, the TMA producer and two warps that only give up their registers:
+// 168 per thread at launch, 208 for the first two groups and 88 for the last make the same sum
+constexpr int kThreads = 384;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRescaleAbove = 8.0f;     // powers of two that a maximum may lag behind
 
@@ -191,265 +193,271 @@ prefill_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
   tc_fence_after_sync();
   const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, *tmem_slot, 0);
 
-  if (warp == 9) {
-    // ------------------------------ TMA producer ------------------------
-    bool ok = true;
-    if (!p.no_loads) {
-      if (lane == 0) {
-        mbar_arrive_expect_tx(q_full, NT * C::kQBytes);   // (a tile without rows is loaded too: nothing of it is stored)
-        for (int i = 0; i < NT; ++i) {
-          const TileAt t = i == 0 ? t0 : t1;
-          for (int x = 0; x < C::kBoxes; ++x)
-            tma_load_2d(smem + i * C::kQBytes + x * (kTile * 128), &map_q, q_full, t.head * D + x * 64, c0 + t.q0);
-        }
-      }
-      int stage = 0;
-      uint32_t phase = 0;
-      for (int it = 0; it < 2 * blocks; ++it) {           // K 0, V 0, K 1, V 1, ...
-        const int j = it >> 1;
-        const bool is_v = (it & 1) != 0;
-        if (!warp_wait(&empty[stage], phase ^ 1u, abort_flag, p.status, kSiteAProducerEmpty)) {
-          ok = false;
-          break;
-        }
-        uint8_t* dst = ring + stage * C::kStageBytes;
-        const bool tail = is_v && (j + 1) * BN > n;        // (once, in the last block of the prompt)
-        uint64_t* bar = tail ? edge : &full[stage];
+  if (warp >= 8) {
+    reg_dealloc<88>();
+    if (warp == 9) {
+      // ------------------------------ TMA producer ------------------------
+      bool ok = true;
+      if (!p.no_loads) {
         if (lane == 0) {
-          mbar_arrive_expect_tx(bar, C::kStageBytes);
-          for (int x = 0; x < C::kBoxes; ++x)
-            tma_load_2d(dst + x * (BN * 128), is_v ? &map_v : &map_k, bar, kv_col + x * 64, c0 + j * BN);
+          mbar_arrive_expect_tx(q_full, NT * C::kQBytes);   // (a tile without rows is loaded too: nothing of it is stored)
+          for (int i = 0; i < NT; ++i) {
+            const TileAt t = i == 0 ? t0 : t1;
+            for (int x = 0; x < C::kBoxes; ++x)
+              tma_load_2d(smem + i * C::kQBytes + x * (kTile * 128), &map_q, q_full, t.head * D + x * 64, c0 + t.q0);
+          }
         }
-        __syncwarp();
-        if (tail) {
-          if (!warp_wait(edge, 0u, abort_flag, p.status, kSiteAProducerEdge)) {
+        int stage = 0;
+        uint32_t phase = 0;
+        for (int it = 0; it < 2 * blocks; ++it) {           // K 0, V 0, K 1, V 1, ...
+          const int j = it >> 1;
+          const bool is_v = (it & 1) != 0;
+          if (!warp_wait(&empty[stage], phase ^ 1u, abort_flag, p.status, kSiteAProducerEmpty)) {
             ok = false;
             break;
           }
-          const int r0 = n - j * BN;                       // the swizzle moves 16-byte pieces inside a row only
-          for (int x = 0; x < C::kBoxes; ++x)
-            for (int i = r0 * 8 + lane; i < BN * 8; i += 32)
-              reinterpret_cast<uint4*>(dst + x * (BN * 128))[i] = make_uint4(0u, 0u, 0u, 0u);
-          fence_proxy_async_smem();
+          uint8_t* dst = ring + stage * C::kStageBytes;
+          const bool tail = is_v && (j + 1) * BN > n;        // (once, in the last block of the prompt)
+          uint64_t* bar = tail ? edge : &full[stage];
+          if (lane == 0) {
+            mbar_arrive_expect_tx(bar, C::kStageBytes);
+            for (int x = 0; x < C::kBoxes; ++x)
+              tma_load_2d(dst + x * (BN * 128), is_v ? &map_v : &map_k, bar, kv_col + x * 64, c0 + j * BN);
+          }
           __syncwarp();
-          if (lane == 0) mbar_arrive(&full[stage]);
-        }
-        if (++stage == C::kStages) {
-          stage = 0;
-          phase ^= 1u;
-        }
-      }
-    }
-    if (!ok) {
-      // copies that this warp started may still be on their way: give them time to land before the CTA ends
-      const long long w0 = clock64();
-      while (clock64() - w0 < (1LL << 22)) {
-      }
-    }
-  } else if (warp == 8) {
-    // ------------------------------ MMA issuer --------------------------
-    constexpr uint32_t idesc_s = umma_idesc_16bit_f32(Num<T>::kFormat, kTile, BN, false);
-    constexpr uint32_t idesc_o = umma_idesc_16bit_f32(Num<T>::kFormat, kTile, D, true);
-    const uint32_t q_addr = smem_u32(smem), ring_addr = smem_u32(ring);
-    // K block j is element 2 j of the ring's sequence, V block j element 2 j + 1
-    auto stage_of = [&](int it) { return it % C::kStages; };
-    auto wait_full = [&](int it) {
-      return warp_wait(&full[stage_of(it)], (it / C::kStages) & 1, abort_flag, p.status, kSiteAMmaFull);
-    };
-    auto scores = [&](int i, int j) {       // S = Q_i K_j^T
-      const uint32_t d = tmem + C::kSCol + (NT == 2 ? i : j & 1) * BN;
-      const uint32_t k = ring_addr + stage_of(2 * j) * C::kStageBytes, q = q_addr + i * C::kQBytes;
-      if (elect_one()) {
-#pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-          const uint32_t in_box = (kk % 4) * 32;
-          umma_16bit_ss(d, umma_desc_k_sw128(q + (kk / 4) * (kTile * 128) + in_box), umma_desc_k_sw128(k + (kk / 4) * (BN * 128) + in_box),
-                        idesc_s, kk > 0 ? 1u : 0u);
-        }
-        umma_commit(&s_full[NT == 2 ? i : j & 1]);
-      }
-      __syncwarp();
-    };
-    auto sums = [&](int i, int j) {         // O_i += P V_j
-      const uint32_t a = tmem + C::kSCol + (NT == 2 ? i : j & 1) * BN;
-      const uint32_t v = ring_addr + stage_of(2 * j + 1) * C::kStageBytes;
-      if (elect_one()) {
-#pragma unroll
-        for (int kk = 0; kk < BN / 16; ++kk)
-          umma_16bit_ts(tmem + C::kOCol + i * D, a + kk * 8, umma_desc_mn_sw128(v + kk * 2048, BN * 128), idesc_o, j > 0 || kk > 0 ? 1u : 0u);
-        umma_commit(&o_done[i]);
-      }
-      __syncwarp();
-    };
-    auto release = [&](int it) {
-      if (elect_one()) umma_commit(&empty[stage_of(it)]);
-      __syncwarp();
-    };
-    auto wait_p = [&](int i, int j) {
-      return warp_wait(&p_full[NT == 2 ? i : j & 1], (NT == 2 ? j : j >> 1) & 1, abort_flag, p.status, kSiteAMmaP);
-    };
-    const int tile_blocks[2] = {t0.blocks, t1.blocks};
-    bool ok = warp_wait(q_full, 0u, abort_flag, p.status, kSiteAMmaQ) && wait_full(0);
-    if (ok) {
-      tc_fence_after_sync();
-#pragma unroll
-      for (int i = 0; i < NT; ++i)
-        if (tile_blocks[i] > 0) scores(i, 0);
-      release(0);
-    }
-    for (int j = 0; ok && j < blocks; ++j) {
-      if (NT == 1 && j + 1 < blocks) {
-        ok = wait_full(2 * j + 2);
-        if (!ok) break;
-        tc_fence_after_sync();
-        scores(0, j + 1);
-        release(2 * j + 2);
-      }
-      ok = wait_full(2 * j + 1);
-#pragma unroll
-      for (int i = 0; i < NT; ++i) {
-        if (!ok) break;
-        if (j < tile_blocks[i]) {
-          ok = wait_p(i, j);
-          if (!ok) break;
-          tc_fence_after_sync();
-          sums(i, j);
-        }
-        if (i == NT - 1) release(2 * j + 1);
-        if (NT == 2 && j + 1 < blocks) {
-          if (i == 0) ok = wait_full(2 * j + 2);
-          if (!ok) break;
-          tc_fence_after_sync();
-          if (j + 1 < tile_blocks[i]) scores(i, j + 1);
-          if (i == 1) release(2 * j + 2);
-        }
-      }
-    }
-  } else if (warp < 4 * NT) {
-    // ------------------------------ softmax: a thread per row -----------
-    const int i = warp >> 2;
-    const TileAt t = i == 0 ? t0 : t1;
-    const int pos = t.q0 + (warp & 3) * 32 + lane;
-    const int lim = min(n, max(pos + 1, prefix));          // keys from here on are masked (rows behind the prompt: any)
-    const int lim_warp = __shfl_sync(0xFFFFFFFFu, lim, 0);
-    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const uint32_t o_at = tmem + lanes + C::kOCol + i * D;
-    const float slope = kMod && p.slopes ? __ldg(p.slopes + t.head) * kLog2e : 0.0f;
-    float m = -INFINITY, l = 0.0f;                         // m: what the row's exponentials are relative to, base 2
-    bool ok = true;
-    for (int j = 0; j < t.blocks; ++j) {
-      const int buf = NT == 2 ? i : j & 1;
-      const uint32_t s_at = tmem + lanes + C::kSCol + buf * BN;
-      ok = warp_wait(&s_full[buf], (NT == 2 ? j : j >> 1) & 1, abort_flag, p.status, kSiteASoftmaxS);
-      if (!ok) break;
-      tc_fence_after_sync();
-      uint32_t s[BN / 32][32];
-#pragma unroll
-      for (int c = 0; c < BN / 32; ++c) tmem_ld_32x32(s_at + c * 32, s[c]);
-      tmem_ld_wait();
-#pragma unroll
-      for (int c = 0; c < BN / 32; ++c) pin32(s[c]);
-      if constexpr (kMod) {
-#pragma unroll
-        for (int c = 0; c < BN / 32; ++c) {
-#pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            float x = __uint_as_float(s[c][e]) * p.scale_log2e;
-            if (p.cap_log2e > 0.0f) {
-              // tanh(x) = 1 - 2 / (1 + e^2x): off by some 2^-22, which the cap multiplies
-              float r;
-              asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + ex2(x * (2.0f * kLog2e))));
-              x = p.cap_log2e * fmaf(-2.0f, r, 1.0f);
+          if (tail) {
+            if (!warp_wait(edge, 0u, abort_flag, p.status, kSiteAProducerEdge)) {
+              ok = false;
+              break;
             }
-            s[c][e] = __float_as_uint(fmaf(-slope, fabsf(static_cast<float>(pos - (j * BN + c * 32 + e))), x));
+            const int r0 = n - j * BN;                       // the swizzle moves 16-byte pieces inside a row only
+            for (int x = 0; x < C::kBoxes; ++x)
+              for (int i = r0 * 8 + lane; i < BN * 8; i += 32)
+                reinterpret_cast<uint4*>(dst + x * (BN * 128))[i] = make_uint4(0u, 0u, 0u, 0u);
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&full[stage]);
+          }
+          if (++stage == C::kStages) {
+            stage = 0;
+            phase ^= 1u;
           }
         }
       }
-      if ((j + 1) * BN > lim_warp) {
+      if (!ok) {
+        // copies that this warp started may still be on their way: give them time to land before the CTA ends
+        const long long w0 = clock64();
+        while (clock64() - w0 < (1LL << 22)) {
+        }
+      }
+    } else if (warp == 8) {
+      // ------------------------------ MMA issuer --------------------------
+      constexpr uint32_t idesc_s = umma_idesc_16bit_f32(Num<T>::kFormat, kTile, BN, false);
+      constexpr uint32_t idesc_o = umma_idesc_16bit_f32(Num<T>::kFormat, kTile, D, true);
+      const uint32_t q_addr = smem_u32(smem), ring_addr = smem_u32(ring);
+      // K block j is element 2 j of the ring's sequence, V block j element 2 j + 1
+      auto stage_of = [&](int it) { return it % C::kStages; };
+      auto wait_full = [&](int it) {
+        return warp_wait(&full[stage_of(it)], (it / C::kStages) & 1, abort_flag, p.status, kSiteAMmaFull);
+      };
+      auto scores = [&](int i, int j) {       // S = Q_i K_j^T
+        const uint32_t d = tmem + C::kSCol + (NT == 2 ? i : j & 1) * BN;
+        const uint32_t k = ring_addr + stage_of(2 * j) * C::kStageBytes, q = q_addr + i * C::kQBytes;
+        if (elect_one()) {
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk) {
+            const uint32_t in_box = (kk % 4) * 32;
+            umma_16bit_ss(d, umma_desc_k_sw128(q + (kk / 4) * (kTile * 128) + in_box), umma_desc_k_sw128(k + (kk / 4) * (BN * 128) + in_box),
+                          idesc_s, kk > 0 ? 1u : 0u);
+          }
+          umma_commit(&s_full[NT == 2 ? i : j & 1]);
+        }
+        __syncwarp();
+      };
+      auto sums = [&](int i, int j) {         // O_i += P V_j
+        const uint32_t a = tmem + C::kSCol + (NT == 2 ? i : j & 1) * BN;
+        const uint32_t v = ring_addr + stage_of(2 * j + 1) * C::kStageBytes;
+        if (elect_one()) {
+#pragma unroll
+          for (int kk = 0; kk < BN / 16; ++kk)
+            umma_16bit_ts(tmem + C::kOCol + i * D, a + kk * 8, umma_desc_mn_sw128(v + kk * 2048, BN * 128), idesc_o, j > 0 || kk > 0 ? 1u : 0u);
+          umma_commit(&o_done[i]);
+        }
+        __syncwarp();
+      };
+      auto release = [&](int it) {
+        if (elect_one()) umma_commit(&empty[stage_of(it)]);
+        __syncwarp();
+      };
+      auto wait_p = [&](int i, int j) {
+        return warp_wait(&p_full[NT == 2 ? i : j & 1], (NT == 2 ? j : j >> 1) & 1, abort_flag, p.status, kSiteAMmaP);
+      };
+      const int tile_blocks[2] = {t0.blocks, t1.blocks};
+      bool ok = warp_wait(q_full, 0u, abort_flag, p.status, kSiteAMmaQ) && wait_full(0);
+      if (ok) {
+        tc_fence_after_sync();
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+          if (tile_blocks[i] > 0) scores(i, 0);
+        release(0);
+      }
+      for (int j = 0; ok && j < blocks; ++j) {
+        if (NT == 1 && j + 1 < blocks) {
+          ok = wait_full(2 * j + 2);
+          if (!ok) break;
+          tc_fence_after_sync();
+          scores(0, j + 1);
+          release(2 * j + 2);
+        }
+        ok = wait_full(2 * j + 1);
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+          if (!ok) break;
+          if (j < tile_blocks[i]) {
+            ok = wait_p(i, j);
+            if (!ok) break;
+            tc_fence_after_sync();
+            sums(i, j);
+          }
+          if (i == NT - 1) release(2 * j + 1);
+          if (NT == 2 && j + 1 < blocks) {
+            if (i == 0) ok = wait_full(2 * j + 2);
+            if (!ok) break;
+            tc_fence_after_sync();
+            if (j + 1 < tile_blocks[i]) scores(i, j + 1);
+            if (i == 1) release(2 * j + 2);
+          }
+        }
+      }
+    }
+  } else {
+    reg_alloc<208>();
+    if (warp < 4 * NT) {
+      // ------------------------------ softmax: a thread per row -----------
+      const int i = warp >> 2;
+      const TileAt t = i == 0 ? t0 : t1;
+      const int pos = t.q0 + (warp & 3) * 32 + lane;
+      const int lim = min(n, max(pos + 1, prefix));          // keys from here on are masked (rows behind the prompt: any)
+      const int lim_warp = __shfl_sync(0xFFFFFFFFu, lim, 0);
+      const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+      const uint32_t o_at = tmem + lanes + C::kOCol + i * D;
+      const float slope = kMod && p.slopes ? __ldg(p.slopes + t.head) * kLog2e : 0.0f;
+      float m = -INFINITY, l = 0.0f;                         // m: what the row's exponentials are relative to, base 2
+      bool ok = true;
+      for (int j = 0; j < t.blocks; ++j) {
+        const int buf = NT == 2 ? i : j & 1;
+        const uint32_t s_at = tmem + lanes + C::kSCol + buf * BN;
+        ok = warp_wait(&s_full[buf], (NT == 2 ? j : j >> 1) & 1, abort_flag, p.status, kSiteASoftmaxS);
+        if (!ok) break;
+        tc_fence_after_sync();
+        uint32_t s[BN / 32][32];
+#pragma unroll
+        for (int c = 0; c < BN / 32; ++c) tmem_ld_32x32(s_at + c * 32, s[c]);
+        tmem_ld_wait();
+#pragma unroll
+        for (int c = 0; c < BN / 32; ++c) pin32(s[c]);
+        if constexpr (kMod) {
+#pragma unroll
+          for (int c = 0; c < BN / 32; ++c) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) {
+              float x = __uint_as_float(s[c][e]) * p.scale_log2e;
+              if (p.cap_log2e > 0.0f) {
+                // tanh(x) = 1 - 2 / (1 + e^2x): off by some 2^-22, which the cap multiplies
+                float r;
+                asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + ex2(x * (2.0f * kLog2e))));
+                x = p.cap_log2e * fmaf(-2.0f, r, 1.0f);
+              }
+              s[c][e] = __float_as_uint(fmaf(-slope, fabsf(static_cast<float>(pos - (j * BN + c * 32 + e))), x));
+            }
+          }
+        }
+        if ((j + 1) * BN > lim_warp) {
+#pragma unroll
+          for (int c = 0; c < BN / 32; ++c) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (j * BN + c * 32 + e >= lim) s[c][e] = 0xFF800000u;   // -inf
+          }
+        }
+        const float f = kMod ? 1.0f : p.scale_log2e;
+        float mx[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) mx[e] = -INFINITY;
 #pragma unroll
         for (int c = 0; c < BN / 32; ++c) {
 #pragma unroll
-          for (int e = 0; e < 32; ++e)
-            if (j * BN + c * 32 + e >= lim) s[c][e] = 0xFF800000u;   // -inf
+          for (int e = 0; e < 32; ++e) mx[e & 3] = fmaxf(mx[e & 3], __uint_as_float(s[c][e]));
         }
+        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * f;
+        // (rows behind the prompt have no say: a prompt's bits do not depend on its neighbours)
+        if (__any_sync(0xFFFFFFFFu, pos < n && (top > m + kRescaleAbove || m == -INFINITY))) {
+          const float m_new = fmaxf(m, top);
+          const float alpha = m_new == -INFINITY ? 1.0f : ex2(m - m_new);   // (every score so far -inf: no weight, not NaN)
+          l *= alpha;
+          m = m_new;
+          if (j > 0) {
+            // the product before is the last one on these sums until this warp's next arrival
+            ok = warp_wait(&o_done[i], (j - 1) & 1, abort_flag, p.status, kSiteASoftmaxO);
+            if (!ok) break;
+            tc_fence_after_sync();
+#pragma unroll 1
+            for (int c = 0; c < D; c += 32) {
+              uint32_t o[32];
+              tmem_ld_32x32(o_at + c, o);
+              tmem_ld_wait();
+              pin32(o);
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+              tmem_st_32x32(o_at + c, o);
+            }
+          }
+        }
+        const float ref = (m == -INFINITY ? 0.0f : m) - Num<T>::kUp;
+        const float2 f2 = make_float2(f, f), ref2 = make_float2(-ref, -ref);
+        float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+#pragma unroll
+        for (int c = 0; c < BN / 32; ++c) {
+          uint32_t w[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            float2 x = make_float2(__uint_as_float(s[c][2 * e]), __uint_as_float(s[c][2 * e + 1]));
+            x = kMod ? __fadd2_rn(x, ref2) : __ffma2_rn(x, f2, ref2);
+            x.x = ex2(x.x);
+            x.y = ex2(x.y);
+            sum[e & 1] = __fadd2_rn(sum[e & 1], x);
+            w[e] = Num<T>::pack(x.x, x.y);
+          }
+          tmem_st_32x16(s_at + c * 16, w);
+        }
+        l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+        tmem_st_wait();
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[buf]);
       }
-      const float f = kMod ? 1.0f : p.scale_log2e;
-      float mx[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) mx[e] = __uint_as_float(s[0][e]);
-#pragma unroll
-      for (int c = 0; c < BN / 32; ++c) {
-#pragma unroll
-        for (int e = c == 0 ? 4 : 0; e < 32; ++e) mx[e & 3] = fmaxf(mx[e & 3], __uint_as_float(s[c][e]));
-      }
-      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * f;
-      // (rows behind the prompt have no say: a prompt's bits do not depend on its neighbours)
-      if (__any_sync(0xFFFFFFFFu, pos < n && (top > m + kRescaleAbove || m == -INFINITY))) {
-        const float m_new = fmaxf(m, top);
-        const float alpha = m_new == -INFINITY ? 1.0f : ex2(m - m_new);   // (every score so far -inf: no weight, not NaN)
-        l *= alpha;
-        m = m_new;
-        if (j > 0) {
-          // the product before is the last one on these sums until this warp's next arrival
-          ok = warp_wait(&o_done[i], (j - 1) & 1, abort_flag, p.status, kSiteASoftmaxO);
-          if (!ok) break;
+      // ---- the row's sums / l
+      if (t.blocks > 0 && ok) {
+        if (warp_wait(&o_done[i], (t.blocks - 1) & 1, abort_flag, p.status, kSiteASoftmaxO)) {
           tc_fence_after_sync();
+          const float inv = 1.0f / l;
+          T* dst = static_cast<T*>(p.out) + (static_cast<int64_t>(c0) + pos) * p.out_stride + static_cast<int64_t>(t.head) * D;
 #pragma unroll 1
           for (int c = 0; c < D; c += 32) {
             uint32_t o[32];
             tmem_ld_32x32(o_at + c, o);
             tmem_ld_wait();
             pin32(o);
+            if (pos < n) {
 #pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-            tmem_st_32x32(o_at + c, o);
-          }
-        }
-      }
-      const float ref = (m == -INFINITY ? 0.0f : m) - Num<T>::kUp;
-      const float2 f2 = make_float2(f, f), ref2 = make_float2(-ref, -ref);
-      float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
-#pragma unroll
-      for (int c = 0; c < BN / 32; ++c) {
-        uint32_t w[16];
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          float2 x = make_float2(__uint_as_float(s[c][2 * e]), __uint_as_float(s[c][2 * e + 1]));
-          x = kMod ? __fadd2_rn(x, ref2) : __ffma2_rn(x, f2, ref2);
-          x.x = ex2(x.x);
-          x.y = ex2(x.y);
-          sum[e & 1] = __fadd2_rn(sum[e & 1], x);
-          w[e] = Num<T>::pack(x.x, x.y);
-        }
-        tmem_st_32x16(s_at + c * 16, w);
-      }
-      l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
-      tmem_st_wait();
-      tc_fence_before_sync();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&p_full[buf]);
-    }
-    // ---- the row's sums / l
-    if (t.blocks > 0 && ok) {
-      if (warp_wait(&o_done[i], (t.blocks - 1) & 1, abort_flag, p.status, kSiteASoftmaxO)) {
-        tc_fence_after_sync();
-        const float inv = 1.0f / l;
-        T* dst = static_cast<T*>(p.out) + (static_cast<int64_t>(c0) + pos) * p.out_stride + static_cast<int64_t>(t.head) * D;
-#pragma unroll 1
-        for (int c = 0; c < D; c += 32) {
-          uint32_t o[32];
-          tmem_ld_32x32(o_at + c, o);
-          tmem_ld_wait();
-          pin32(o);
-          if (pos < n) {
-#pragma unroll
-            for (int e = 0; e < 32; e += 8) {
-              uint4 w;
-              w.x = Num<T>::pack(__uint_as_float(o[e]) * inv, __uint_as_float(o[e + 1]) * inv);
-              w.y = Num<T>::pack(__uint_as_float(o[e + 2]) * inv, __uint_as_float(o[e + 3]) * inv);
-              w.z = Num<T>::pack(__uint_as_float(o[e + 4]) * inv, __uint_as_float(o[e + 5]) * inv);
-              w.w = Num<T>::pack(__uint_as_float(o[e + 6]) * inv, __uint_as_float(o[e + 7]) * inv);
-              *reinterpret_cast<uint4*>(dst + c + e) = w;
+              for (int e = 0; e < 32; e += 8) {
+                uint4 w;
+                w.x = Num<T>::pack(__uint_as_float(o[e]) * inv, __uint_as_float(o[e + 1]) * inv);
+                w.y = Num<T>::pack(__uint_as_float(o[e + 2]) * inv, __uint_as_float(o[e + 3]) * inv);
+                w.z = Num<T>::pack(__uint_as_float(o[e + 4]) * inv, __uint_as_float(o[e + 5]) * inv);
+                w.w = Num<T>::pack(__uint_as_float(o[e + 6]) * inv, __uint_as_float(o[e + 7]) * inv);
+                *reinterpret_cast<uint4*>(dst + c + e) = w;
+              }
             }
           }
         }
