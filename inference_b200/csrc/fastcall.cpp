@@ -247,9 +247,181 @@ PyObject* paged_attn_decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+bool integer(PyObject* o, long* v) {
+  if (!PyLong_CheckExact(o)) return false;
+  int overflow = 0;
+  *v = PyLong_AsLongAndOverflow(o, &overflow);
+  return overflow == 0;
+}
+bool real(PyObject* o, double* v) {
+  if (!PyFloat_CheckExact(o)) {
+    long l;
+    if (!integer(o, &l)) return false;
+    *v = static_cast<double>(l);
+    return true;
+  }
+  *v = PyFloat_AS_DOUBLE(o);
+  return true;
+}
+// an argument that may be None: true where it is, or where it is a plain tensor of this type and shape
+bool optional(PyObject* o, c10::DeviceIndex dev, at::ScalarType type, at::IntArrayRef sizes, const void** ptr) {
+  *ptr = nullptr;
+  if (o == Py_None) return true;
+  const at::Tensor* t = tensor(o);
+  if (!plain(t, dev) || t->scalar_type() != type || t->sizes() != sizes) return false;
+  *ptr = t->data_ptr();
+  return true;
+}
+bool is(const at::Tensor* t, c10::DeviceIndex dev, at::ScalarType type, at::IntArrayRef sizes) {
+  return plain(t, dev) && t->scalar_type() == type && t->sizes() == sizes;
+}
+// [tokens, rows, dim] whose rows of a token are contiguous: the stride of a token, or -1
+int64_t token_stride(const at::Tensor* t, c10::DeviceIndex dev, at::ScalarType type, at::IntArrayRef sizes) {
+  if (!t || !t->is_cuda() || t->device().index() != dev || t->scalar_type() != type || t->sizes() != sizes || t->size(0) == 0 ||
+      t->stride(2) != 1 || (t->size(1) > 1 && t->stride(1) != t->size(2))) {
+    return -1;
+  }
+  return t->size(0) > 1 ? t->stride(0) : t->size(1) * t->size(2);
+}
+bool fits(std::initializer_list<int64_t> sizes) {
+  for (const int64_t v : sizes)
+    if (v > 0x7FFFFFFF) return false;
+  return true;
+}
+const int32_t* ints(const at::Tensor* t) { return static_cast<const int32_t*>(t->data_ptr()); }
+
+// rope_append(q, k, v, k_cache, v_cache, k_scales, v_scales, block_tables, seq_lens, rotary_dim, base, yarn_factor, cu_seqlens or
+// None, k_out or None); k_scales None: caches of q's type
+PyObject* rope_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  long rotary;
+  double base, yarn;
+  if (n != 14 || !integer(a[9], &rotary) || rotary < 0 || rotary > 0x7FFFFFFF || !real(a[10], &base) || !real(a[11], &yarn)) Py_RETURN_NONE;
+  const bool fp8 = a[5] != Py_None;
+  const at::Tensor *q = tensor(a[0]), *k = tensor(a[1]), *v = tensor(a[2]), *kc = tensor(a[3]), *vc = tensor(a[4]);
+  const at::Tensor *bt = tensor(a[7]), *sl = tensor(a[8]), *ko = a[13] == Py_None ? nullptr : tensor(a[13]);
+  if (!q || !k || !kc || !q->is_cuda() || q->dim() != 3 || k->dim() != 3 || !bt || bt->dim() != 2 || kc->dim() != 4) Py_RETURN_NONE;
+  const c10::DeviceIndex dev = c10::cuda::current_device();
+  const at::ScalarType t = q->scalar_type();
+  const int dt = code_of(t);
+  const int64_t tokens = q->size(0), heads = q->size(1), dim = q->size(2), kv = k->size(1);
+  const int64_t batch = bt->size(0), per = bt->size(1), blocks = kc->size(0), block = kc->size(1);
+  if (dt < 0 || !fits({heads, kv, dim, batch, per, blocks, block})) Py_RETURN_NONE;
+  const int64_t qs = token_stride(q, dev, t, {tokens, heads, dim}), ks = token_stride(k, dev, t, {tokens, kv, dim});
+  const int64_t vs = token_stride(v, dev, t, {tokens, kv, dim}), kos = ko ? token_stride(ko, dev, t, {tokens, kv, dim}) : 0;
+  const at::ScalarType ct = fp8 ? at::kByte : t;
+  if (qs < 0 || ks < 0 || vs < 0 || kos < 0 || (a[13] != Py_None && !ko) || !is(kc, dev, ct, {blocks, block, kv, dim}) ||
+      !is(vc, dev, ct, {blocks, block, kv, dim}) || !is(bt, dev, at::kInt, {batch, per}) || !is(sl, dev, at::kInt, {batch})) {
+    Py_RETURN_NONE;
+  }
+  const void *kss, *vss, *cu;
+  if (!optional(a[5], dev, at::kFloat, {blocks, kv}, &kss) || !optional(a[6], dev, at::kFloat, {blocks, kv}, &vss) ||
+      !optional(a[12], dev, at::kInt, {batch + 1}, &cu)) {
+    Py_RETURN_NONE;
+  }
+  at::Tensor out;
+  int rc;
+  {
+    pybind11::gil_scoped_release unlocked;
+    out = make({tokens, heads, dim}, *q, t);
+    void* const ko_ptr = ko ? ko->data_ptr() : nullptr;
+    const auto i32 = [](int64_t x) { return static_cast<int32_t>(x); };
+    if (fp8) {
+      rc = inferop_rope_append_kv_fp8(out.data_ptr(), heads * dim, ko_ptr, kos, kc->data_ptr(), vc->data_ptr(), const_cast<void*>(kss),
+                                      const_cast<void*>(vss), q->data_ptr(), qs, k->data_ptr(), ks, v->data_ptr(), vs, ints(bt), ints(sl),
+                                      static_cast<const int32_t*>(cu), dt, tokens, i32(batch), i32(heads), i32(kv), i32(dim), i32(rotary),
+                                      i32(block), i32(blocks), i32(per), base, yarn, stream_of(dev));
+    } else {
+      rc = inferop_rope_append_kv(out.data_ptr(), heads * dim, ko_ptr, kos, kc->data_ptr(), vc->data_ptr(), q->data_ptr(), qs,
+                                  k->data_ptr(), ks, v->data_ptr(), vs, ints(bt), ints(sl), static_cast<const int32_t*>(cu), dt, tokens,
+                                  i32(batch), i32(heads), i32(kv), i32(dim), i32(rotary), i32(block), i32(blocks), i32(per), base, yarn,
+                                  stream_of(dev));
+    }
+  }
+  if (rc != INFEROP_OK) return PyLong_FromLong(rc);
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+// paged_attn_decode_scored(q, k_cache, v_cache, k_scales, v_scales, block_tables, seq_lens, scale, softcap, alibi_slopes or None);
+// k_scales None: caches of q's type
+PyObject* paged_attn_decode_scored(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  float scale, cap;
+  if (n != 10 || !number(a[7], &scale) || !number(a[8], &cap)) Py_RETURN_NONE;
+  const bool fp8 = a[3] != Py_None;
+  const at::Tensor *q = tensor(a[0]), *kc = tensor(a[1]), *vc = tensor(a[2]), *bt = tensor(a[5]), *sl = tensor(a[6]);
+  c10::DeviceIndex dev;
+  if (!leads(q, &dev) || q->dim() != 3 || !kc || kc->dim() != 4 || !bt || bt->dim() != 2) Py_RETURN_NONE;
+  const at::ScalarType t = q->scalar_type(), ct = fp8 ? at::kByte : t;
+  const int dt = code_of(t);
+  const int64_t batch = q->size(0), heads = q->size(1), dim = q->size(2), per = bt->size(1);
+  const int64_t blocks = kc->size(0), block = kc->size(1), kv = kc->size(2);
+  if (dt < (fp8 ? 1 : 0) || !fits({batch, heads, dim, per, blocks, block, kv})) Py_RETURN_NONE;
+  const void *kss, *vss, *slopes;
+  if (!is(kc, dev, ct, {blocks, block, kv, dim}) || !is(vc, dev, ct, {blocks, block, kv, dim}) || !is(bt, dev, at::kInt, {batch, per}) ||
+      !is(sl, dev, at::kInt, {batch}) || !optional(a[3], dev, at::kFloat, {blocks, kv}, &kss) ||
+      !optional(a[4], dev, at::kFloat, {blocks, kv}, &vss) || !optional(a[9], dev, at::kFloat, {heads}, &slopes)) {
+    Py_RETURN_NONE;
+  }
+  at::Tensor out;
+  int rc;
+  {
+    pybind11::gil_scoped_release unlocked;
+    out = make(q->sizes(), *q, t);
+    const auto i32 = [](int64_t x) { return static_cast<int32_t>(x); };
+    const float* sl_ptr = static_cast<const float*>(slopes);
+    if (fp8) {
+      rc = inferop_paged_attn_decode_fp8(out.data_ptr(), q->data_ptr(), kc->data_ptr(), vc->data_ptr(), kss, vss, ints(bt), ints(sl), dt,
+                                         i32(batch), i32(heads), i32(kv), i32(dim), i32(block), i32(blocks), i32(per), scale, cap, sl_ptr,
+                                         stream_of(dev));
+    } else {
+      rc = inferop_paged_attn_decode_scored(out.data_ptr(), q->data_ptr(), kc->data_ptr(), vc->data_ptr(), ints(bt), ints(sl), dt, i32(batch),
+                                            i32(heads), i32(kv), i32(dim), i32(block), i32(per), scale, cap, sl_ptr, stream_of(dev));
+    }
+  }
+  if (rc != INFEROP_OK) return PyLong_FromLong(rc);
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+// prefill_attn(q, k, v, cu_seqlens, scale, softcap, alibi_slopes or None, prefix_lens or None)
+PyObject* prefill_attn(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  float scale, cap;
+  if (n != 8 || !number(a[4], &scale) || !number(a[5], &cap)) Py_RETURN_NONE;
+  const at::Tensor *q = tensor(a[0]), *k = tensor(a[1]), *v = tensor(a[2]), *cu = tensor(a[3]);
+  if (!q || !q->is_cuda() || q->dim() != 3 || !k || k->dim() != 3 || !cu || cu->dim() != 1 || cu->size(0) < 2) Py_RETURN_NONE;
+  const c10::DeviceIndex dev = c10::cuda::current_device();
+  const at::ScalarType t = q->scalar_type();
+  const int dt = code_of(t);
+  const int64_t tokens = q->size(0), heads = q->size(1), dim = q->size(2), kv = k->size(1), batch = cu->size(0) - 1;
+  if (dt < 1 || !fits({heads, kv, dim, batch})) Py_RETURN_NONE;
+  const int64_t qs = token_stride(q, dev, t, {tokens, heads, dim}), ks = token_stride(k, dev, t, {tokens, kv, dim});
+  const int64_t vs = token_stride(v, dev, t, {tokens, kv, dim});
+  const void *slopes, *prefix;
+  if (qs < 0 || ks < 0 || vs < 0 || !is(cu, dev, at::kInt, {batch + 1}) || !optional(a[6], dev, at::kFloat, {heads}, &slopes) ||
+      !optional(a[7], dev, at::kInt, {batch}, &prefix)) {
+    Py_RETURN_NONE;
+  }
+  at::Tensor out;
+  int rc;
+  {
+    pybind11::gil_scoped_release unlocked;
+    out = make({tokens, heads, dim}, *q, t);
+    rc = inferop_prefill_attn(out.data_ptr(), heads * dim, q->data_ptr(), qs, k->data_ptr(), ks, v->data_ptr(), vs, ints(cu),
+                              static_cast<const int32_t*>(prefix), dt, tokens, static_cast<int32_t>(batch), static_cast<int32_t>(heads),
+                              static_cast<int32_t>(kv), static_cast<int32_t>(dim), scale, cap, static_cast<const float*>(slopes),
+                              stream_of(dev));
+  }
+  if (rc != INFEROP_OK) return PyLong_FromLong(rc);
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
 #define FAST(f) {#f, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {FAST(quant), FAST(gemm), FAST(gemm_fused_quant), FAST(rmsnorm_quant), FAST(rope_neox),
-                         FAST(paged_attn_decode), {nullptr, nullptr, 0, nullptr}};
+                         FAST(paged_attn_decode), FAST(rope_append), FAST(paged_attn_decode_scored), FAST(prefill_attn), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_fastcall", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

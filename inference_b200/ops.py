@@ -453,6 +453,10 @@ def _on_device(like: torch.Tensor, **tensors) -> None:
 
 def _append(what, q, k, v, k_cache, v_cache, scales, block_tables, seq_lens, rotary_dim, base, yarn_factor, cu_seqlens, q_out, k_out,
             stream):
+    if q_out is None and stream is None and \
+            _made(r := fast.rope_append(q, k, v, k_cache, v_cache, *(scales or (None, None)), block_tables, seq_lens, rotary_dim, base,
+                                        yarn_factor, cu_seqlens, k_out), what):
+        return r
     if q.dim() != 3 or k.dim() != 3 or k_cache.dim() != 4 or block_tables.dim() != 2 or q.dtype not in _TORCH2CODE:
         raise ValueError("q must be [tokens, heads, dim] (fp32/fp16/bf16), k and v [tokens, kv_heads, dim], the caches [blocks, "
                          "block_size, kv_heads, dim] and block_tables [batch, max_blocks]")
@@ -525,9 +529,13 @@ def paged_attn_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
     softcap > 0: scores are softcap * tanh(score / softcap).  alibi_slopes fp32 [heads]: then minus the head's slope times a
     token's distance from the last one."""
     scored = alibi_slopes is not None or softcap != 0.0
-    if not scored and out is None and stream is None and \
-            _made(r := fast.paged_attn_decode(q, k_cache, v_cache, block_tables, seq_lens, scale), "paged_attn_decode"):
-        return r
+    if out is None and stream is None:
+        if scored:
+            r = fast.paged_attn_decode_scored(q, k_cache, v_cache, None, None, block_tables, seq_lens, scale, softcap, alibi_slopes)
+        else:
+            r = fast.paged_attn_decode(q, k_cache, v_cache, block_tables, seq_lens, scale)
+        if _made(r, "paged_attn_decode"):
+            return r
     for t, name in ((q, "q"), (k_cache, "k_cache"), (v_cache, "v_cache"), (block_tables, "block_tables"),
                     (seq_lens, "seq_lens")):
         _dev_tensor(t, name)
@@ -559,6 +567,10 @@ def paged_attn_decode_fp8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch
     """paged_attn_decode over 8-bit caches (rope_append_kv_fp8): k_cache / v_cache uint8 (E4M3 bytes) [blocks, block_size,
     kv_heads, dim], block_size a multiple of 16, scales fp32 [blocks, kv_heads]; q fp16 or bf16.  Tokens whose block-table entry
     is not a block have no weight."""
+    if out is None and stream is None and \
+            _made(r := fast.paged_attn_decode_scored(q, k_cache, v_cache, k_scales, v_scales, block_tables, seq_lens, scale, softcap,
+                                                     alibi_slopes), "paged_attn_decode_fp8"):
+        return r
     if q.dim() != 3 or q.dtype not in (torch.float16, torch.bfloat16) or k_cache.dim() != 4 or block_tables.dim() != 2:
         raise ValueError("q must be fp16 or bf16 [batch, heads, dim], the caches [blocks, block_size, kv_heads, dim] and block_tables "
                          "[batch, max_blocks]")
@@ -590,6 +602,9 @@ def prefill_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: 
     cu_seqlens int32 [batch + 1]: prompt b is rows cu_seqlens[b] .. cu_seqlens[b + 1] - 1; other rows of `out` are left as they
     were.  Causal; prefix_lens int32 [batch]: every token of a prompt sees its first so many.  softcap and alibi_slopes as in
     paged_attn_decode."""
+    if out is None and stream is None and \
+            _made(r := fast.prefill_attn(q, k, v, cu_seqlens, scale, softcap, alibi_slopes, prefix_lens), "prefill_attn"):
+        return r
     if q.dim() != 3 or k.dim() != 3 or cu_seqlens.dim() != 1 or q.dtype not in (torch.float16, torch.bfloat16):
         raise ValueError("q must be fp16 or bf16 [tokens, heads, dim], k and v [tokens, kv_heads, dim], cu_seqlens [batch + 1]")
     tokens, heads, dim = q.shape
