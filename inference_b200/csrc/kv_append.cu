@@ -13,10 +13,15 @@
 // lost 6e-3 rad by position 1e5.  One fp64 product per token and pair, shared by all heads through shared memory.
 //
 // E4M3: a scale belongs to a cache block and a KV head, so the unit of work is a block, and all of a call's tokens in it
-// belong to one CTA, a warp per head and kind (K, V).  Scales are powers of two: a floating format loses nothing by them
+// belong to one CTA, a warp per head and kind (K, V).  The rows are staged in shared memory and gone through twice, for the
+// maximum and for the bytes: with the rows or the rotated values in registers instead, half as many warps fit an SM, and
+// 16384 tokens took 105 to 116 us for 92.  Scales are powers of two: a floating format loses nothing by them
 // (a scale that fits closer would move the values inside a binade), and when a later token needs a larger one, the
 // tokens already there move to it without another rounding (but for E4M3's subnormals).  The values that are quantised
 // are the rotated ones in fp32.
+//
+// Measured (B200): 16384 tokens of 32 + 2 x 8 heads of 128, bf16, with k_out: 75 us = 5.8 TB/s, into E4M3 caches 85 us = 4.8
+// TB/s; one token each of 8 sequences 3.3 us, of 128 sequences into E4M3 caches 5.5 us (launches in a graph).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -24,17 +29,24 @@
 #include <math.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "internal.h"
+#include "quant_math.cuh"
 #include "ragged.cuh"
 
 namespace ib200 {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 128;      // 16-bit and fp32 caches: a warp per token
 constexpr int kWarps = kThreads / 32;
-constexpr int kItems = 4;          // vector pairs of a thread in flight
+constexpr int kItems = 2;          // vector pairs of a lane in flight (1, 3, 4 or two sets of 1 to 3 were up to a quarter slower)
+constexpr int kWarpsWanted = 148 * 16;
+constexpr int kFp8Threads = 256;   // E4M3 caches: a CTA per block
+constexpr int kFp8Warps = kFp8Threads / 32;
 constexpr int kMaxHalf = 128;      // rotary_dim up to 256, the largest head
-constexpr int kMaxTile = 16;       // tokens of a CTA that share a table of angles
+constexpr int kMaxTile = 16;       // tokens of a block that are handled at a time
+constexpr int kMaxJobBytes = 8192; // ... and bytes of a head of theirs
 constexpr float kMinScale = 7.888609052210118e-31f;   // 2^-100: the scale of a block without a non-zero value
 
 struct AppendParams {
@@ -47,27 +59,11 @@ struct AppendParams {
   int64_t tokens;
   int batch, heads, kv_heads, dim, half, block_size, max_blocks, num_blocks;
   int pairs_log2;                  // log2 of the vector pairs of a head
-  int tile;                        // tokens per CTA of the token role
-  int kv_ctas;                     // E4M3: CTAs of the block role, in front of the others
+  int parts;                       // warps that share a token's heads
+  int chunk;                       // E4M3: tokens that are handled at a time
+  uint32_t kv_ctas;                // E4M3: CTAs of the block role
   double turns[kMaxHalf];          // frequency of pair j in turns per position
 };
-
-template <typename T>
-__device__ __forceinline__ float to_f32(T v);
-template <>
-__device__ __forceinline__ float to_f32(float v) { return v; }
-template <>
-__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
-template <>
-__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
-template <typename T>
-__device__ __forceinline__ T from_f32(float v);
-template <>
-__device__ __forceinline__ float from_f32(float v) { return v; }
-template <>
-__device__ __forceinline__ __half from_f32(float v) { return __float2half_rn(v); }
-template <>
-__device__ __forceinline__ __nv_bfloat16 from_f32(float v) { return __float2bfloat16_rn(v); }
 
 // V elements that are read and written together: 16 bytes, or one element where alignment or the rotary size ask for it
 template <typename T, int V>
@@ -78,6 +74,47 @@ template <int V>
 struct alignas(V) Bytes {
   uint8_t e[V];
 };
+
+// A vector as floats and back, rounded once; 16-bit elements two at a time.
+template <typename T, int V>
+__device__ __forceinline__ void widen(const Vec<T, V>& v, float (&x)[V]) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) x[e] = v.e[e];
+  } else if constexpr (V % 2 == 0) {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(&v);
+#pragma unroll
+    for (int e = 0; e < V; e += 2) {
+      const float2 f = widen2<T>(w[e / 2]);
+      x[e] = f.x;
+      x[e + 1] = f.y;
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < V; ++e) x[e] = static_cast<float>(v.e[e]);
+  }
+}
+template <typename T, int V>
+__device__ __forceinline__ Vec<T, V> narrow(const float (&x)[V]) {
+  Vec<T, V> v;
+  if constexpr (sizeof(T) == 2 && V % 2 == 0) {
+    uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+    for (int e = 0; e < V; e += 2) {
+      if constexpr (std::is_same<T, __half>::value) {
+        const __half2 h = __floats2half2_rn(x[e], x[e + 1]);
+        w[e / 2] = *reinterpret_cast<const uint32_t*>(&h);
+      } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(x[e], x[e + 1]);
+        w[e / 2] = *reinterpret_cast<const uint32_t*>(&h);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < V; ++e) v.e[e] = static_cast<T>(x[e]);
+  }
+  return v;
+}
 
 // where a token lies: its position (-1: nobody's token) and its cache row (-1: none)
 struct Place {
@@ -129,118 +166,118 @@ __device__ __forceinline__ PairOf pair_of(const AppendParams& p, int i) {
   return {2 * i, 2 * i + 1, false};
 }
 
-// x0, x1 <- the pair turned; cs: this token's table
-template <typename T, int V>
-__device__ __forceinline__ void turn(const Vec<T, V>& a, const Vec<T, V>& b, bool turned, const float2* cs, int j, float (&x0)[V],
-                                     float (&x1)[V]) {
+// a pair of vectors turned
+template <int V>
+__device__ __forceinline__ void turn(const float2 (&cs)[V], float (&x0)[V], float (&x1)[V]) {
 #pragma unroll
   for (int e = 0; e < V; ++e) {
-    const float f0 = to_f32<T>(a.e[e]), f1 = to_f32<T>(b.e[e]);
-    if (turned) {
-      const float2 c = cs[j * V + e];
-      x0[e] = f0 * c.x - f1 * c.y;
-      x1[e] = f1 * c.x + f0 * c.y;
-    } else {
-      x0[e] = f0;
-      x1[e] = f1;
-    }
+    const float f0 = x0[e], f1 = x1[e];
+    x0[e] = f0 * cs[e].x - f1 * cs[e].y;
+    x1[e] = f1 * cs[e].x + f0 * cs[e].y;
   }
 }
-template <typename T, int V>
-__device__ __forceinline__ Vec<T, V> narrow(const float (&x)[V]) {
-  Vec<T, V> out;
-#pragma unroll
-  for (int e = 0; e < V; ++e) out.e[e] = from_f32<T>(x[e]);
-  return out;
-}
 
-// ---- a CTA of p.tile tokens: heads [0, heads) are q's, then kv_heads of k, then kv_heads of v (kStore; else q alone)
+// ---- a warp with one token, or with one of p.parts shares of its heads: heads [0, heads) are q's, then kv_heads of k, then
+// kv_heads of v (kStore; else q alone).  Every head has the same pairs, so a lane has one pair (V > 1: a head has at most 32),
+// and with it the angles of its V elements in registers, for all the heads that it sees.  (A CTA of a few tokens with one
+// table in shared memory, read for every head, took 57 us for 8192 tokens of 28 + 2 x 4 heads of 128, fp16; this form 32.)
 template <typename T, int V, bool kStore>
-__device__ __forceinline__ void token_role(const AppendParams& p, int64_t cta, float2* cs) {
-  __shared__ Place places[kMaxTile];
-  const int64_t t0 = cta * p.tile;
-  const int n = static_cast<int>(min(static_cast<int64_t>(p.tile), p.tokens - t0));
-  const int per_token = p.heads + (kStore ? 2 * p.kv_heads : 0);
-  const int total = (n * per_token) << p.pairs_log2;
-  const int mask = (1 << p.pairs_log2) - 1;
+__device__ __forceinline__ void token_role(const AppendParams& p, int64_t unit, float2* cs) {
+  const int lane = threadIdx.x & 31;
+  const int64_t t = unit / p.parts;
+  if (t >= p.tokens) return;
+  const int part = static_cast<int>(unit - t * p.parts);
+  const int all = p.heads + (kStore ? 2 * p.kv_heads : 0), share = (all + p.parts - 1) / p.parts;
+  const int first = part * share, last = min(all, first + share);
+  const int pairs = 1 << p.pairs_log2;
+  // item i of the share: pair i % pairs of head first + i / pairs
+  const int total = (last - first) << p.pairs_log2;
 
   Vec<T, V> a[kItems], b[kItems];
-  auto source = [&](int tok, int h) -> const T* {
-    const int64_t t = t0 + tok;
-    if (h < p.heads) return static_cast<const T*>(p.q) + t * p.q_stride + static_cast<int64_t>(h) * p.dim;
-    h -= p.heads;
-    if (h < p.kv_heads) return static_cast<const T*>(p.k) + t * p.k_stride + static_cast<int64_t>(h) * p.dim;
-    return static_cast<const T*>(p.v) + t * p.v_stride + static_cast<int64_t>(h - p.kv_heads) * p.dim;
-  };
   auto load = [&](int base) {
 #pragma unroll
     for (int i = 0; i < kItems; ++i) {
-      const int it = base + i * kThreads + threadIdx.x;
+      const int it = base + i * 32 + lane;
       if (it < total) {
-        const int th = it >> p.pairs_log2, tok = th / per_token;
-        const PairOf pr = pair_of<V>(p, it & mask);
-        const Vec<T, V>* src = reinterpret_cast<const Vec<T, V>*>(source(tok, th - tok * per_token));
-        a[i] = src[pr.a];
-        b[i] = src[pr.b];
+        int h = first + (it >> p.pairs_log2);
+        const T* src = static_cast<const T*>(p.q) + t * p.q_stride;
+        if (kStore && h >= p.heads) {
+          h -= p.heads;
+          src = static_cast<const T*>(p.k) + t * p.k_stride;
+          if (h >= p.kv_heads) {
+            h -= p.kv_heads;
+            src = static_cast<const T*>(p.v) + t * p.v_stride;
+          }
+        }
+        const PairOf pr = pair_of<V>(p, it & (pairs - 1));
+        const Vec<T, V>* row = reinterpret_cast<const Vec<T, V>*>(src + h * p.dim);
+        a[i] = row[pr.a];
+        b[i] = row[pr.b];
       }
     }
   };
   load(0);
-  const int warp = threadIdx.x >> 5;
-  for (int tok = warp; tok < n; tok += kWarps) {
-    const Place at = place_of(p, t0 + tok);
-    if ((threadIdx.x & 31) == 0) places[tok] = at;
-    for (int j = threadIdx.x & 31; j < p.half; j += 32) cs[tok * p.half + j] = turn_of(p, at.pos, j);
+  const Place at = place_of(p, t);
+  if (at.pos < 0) return;
+  for (int j = lane; j < p.half; j += 32) cs[j] = turn_of(p, at.pos, j);
+  __syncwarp();
+  float2 turns[V];
+  const PairOf mine = pair_of<V>(p, lane & (pairs - 1));
+  if (V > 1 && mine.turned) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) turns[e] = cs[(lane & (pairs - 1)) * V + e];
   }
-  __syncthreads();
-  for (int base = 0; base < total; base += kItems * kThreads) {
+  for (int base = 0; base < total; base += kItems * 32) {
     if (base > 0) load(base);
 #pragma unroll
     for (int i = 0; i < kItems; ++i) {
-      const int it = base + i * kThreads + threadIdx.x;
-      if (it >= total) continue;
-      const int th = it >> p.pairs_log2, tok = th / per_token, j = it & mask;
-      int h = th - tok * per_token;
-      const Place at = places[tok];
-      if (at.pos < 0) continue;
-      const PairOf pr = pair_of<V>(p, j);
-      const int64_t t = t0 + tok;
-      if (h >= p.heads + p.kv_heads) {   // v: as it is
-        if (at.row < 0) continue;
-        h -= p.heads + p.kv_heads;
-        Vec<T, V>* dst = reinterpret_cast<Vec<T, V>*>(static_cast<T*>(p.v_cache) + (at.row * p.kv_heads + h) * p.dim);
-        dst[pr.a] = a[i];
-        dst[pr.b] = b[i];
-        continue;
-      }
-      float x0[V], x1[V];
-      turn<T, V>(a[i], b[i], pr.turned, cs + tok * p.half, j, x0, x1);
-      const Vec<T, V> y0 = narrow<T, V>(x0), y1 = narrow<T, V>(x1);
-      T *first = nullptr, *second = nullptr;
-      if (h < p.heads) {
-        first = static_cast<T*>(p.q_out) + t * p.q_out_stride + static_cast<int64_t>(h) * p.dim;
-      } else {
+      const int it = base + i * 32 + lane;
+      if (it >= total) break;
+      int h = first + (it >> p.pairs_log2);
+      const int j = it & (pairs - 1);
+      const PairOf pr = V > 1 ? mine : pair_of<V>(p, j);
+      T *to = static_cast<T*>(p.q_out) + t * p.q_out_stride, *also = nullptr;
+      bool turned = pr.turned;
+      if (kStore && h >= p.heads) {
         h -= p.heads;
-        if (at.row >= 0) first = static_cast<T*>(p.k_cache) + (at.row * p.kv_heads + h) * p.dim;
-        if (p.k_out) second = static_cast<T*>(p.k_out) + t * p.k_out_stride + static_cast<int64_t>(h) * p.dim;
+        to = at.row < 0 ? nullptr : static_cast<T*>(p.k_cache) + at.row * p.kv_heads * p.dim;
+        also = p.k_out ? static_cast<T*>(p.k_out) + t * p.k_out_stride : nullptr;
+        if (h >= p.kv_heads) {
+          h -= p.kv_heads;
+          to = at.row < 0 ? nullptr : static_cast<T*>(p.v_cache) + at.row * p.kv_heads * p.dim;
+          also = nullptr;
+          turned = false;
+        }
       }
-      if (first) {
-        reinterpret_cast<Vec<T, V>*>(first)[pr.a] = y0;
-        reinterpret_cast<Vec<T, V>*>(first)[pr.b] = y1;
+      if (turned) {
+        if (V == 1) turns[0] = cs[j];
+        float x0[V], x1[V];
+        widen<T, V>(a[i], x0);
+        widen<T, V>(b[i], x1);
+        turn<V>(turns, x0, x1);
+        a[i] = narrow<T, V>(x0);
+        b[i] = narrow<T, V>(x1);
       }
-      if (second) {
-        reinterpret_cast<Vec<T, V>*>(second)[pr.a] = y0;
-        reinterpret_cast<Vec<T, V>*>(second)[pr.b] = y1;
+      if (to) {
+        Vec<T, V>* d = reinterpret_cast<Vec<T, V>*>(to + h * p.dim);
+        d[pr.a] = a[i];
+        d[pr.b] = b[i];
+      }
+      if (also) {
+        Vec<T, V>* d = reinterpret_cast<Vec<T, V>*>(also + h * p.dim);
+        d[pr.a] = a[i];
+        d[pr.b] = b[i];
       }
     }
   }
 }
 
 template <typename T, int V>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, 8)
 append_kernel(const __grid_constant__ AppendParams p) {
-  extern __shared__ float2 cs[];
-  token_role<T, V, true>(p, blockIdx.x, cs);
+  extern __shared__ __align__(16) uint8_t smem[];
+  const int warp = threadIdx.x >> 5;
+  token_role<T, V, true>(p, static_cast<int64_t>(blockIdx.x) * kWarps + warp, reinterpret_cast<float2*>(smem) + warp * p.half);
 }
 
 // ------------------------------------------------------------------------------------------------ E4M3 caches
@@ -250,9 +287,19 @@ __device__ __forceinline__ float scale_for(float amax) {
   const int e = static_cast<int>(u >> 23) - 8;
   return fmaxf(e > 0 ? __uint_as_float(static_cast<uint32_t>(e) << 23) : 0.0f, kMinScale);
 }
-// x / s as an E4M3 byte (1 / s is exact): infinities become +-448, NaN stays NaN
-__device__ __forceinline__ uint8_t quantised(float x, float inv) {
-  return static_cast<uint8_t>(__nv_cvt_float_to_fp8(x * inv, __NV_SATFINITE, __NV_E4M3));
+// x / s as E4M3 bytes (1 / s is exact): infinities become +-448, NaN stays NaN
+template <int V>
+__device__ __forceinline__ Bytes<V> quantised(const float (&x)[V], float inv) {
+  Bytes<V> y;
+  if constexpr (V % 4 == 0) {
+    uint32_t* w = reinterpret_cast<uint32_t*>(&y);
+#pragma unroll
+    for (int e = 0; e < V; e += 4) w[e / 4] = cvt2(x[e] * inv, x[e + 1] * inv) | (cvt2(x[e + 2] * inv, x[e + 3] * inv) << 16);
+  } else {
+#pragma unroll
+    for (int e = 0; e < V; ++e) y.e[e] = static_cast<uint8_t>(__nv_cvt_float_to_fp8(x[e] * inv, __NV_SATFINITE, __NV_E4M3));
+  }
+  return y;
 }
 __device__ __forceinline__ float value_of(uint8_t byte) {
   return __half2float(__half(__nv_cvt_fp8_to_halfraw(byte, __NV_E4M3)));
@@ -298,14 +345,51 @@ __device__ __forceinline__ void block_role(const AppendParams& p, int64_t item, 
   if (row0 < 0 && p.k_out == nullptr) return;
   const int off = pos0 - j * p.block_size;
   const int64_t blk = row0 < 0 ? 0 : row0 / p.block_size;
-  const int mask = (1 << p.pairs_log2) - 1;
-  const int chunks = (n + kMaxTile - 1) / kMaxTile;
+  const int pairs = 1 << p.pairs_log2, mask = pairs - 1;
+  const int chunks = (n + p.chunk - 1) / p.chunk;
 
-  auto table = [&](int c) {   // angles of a chunk's tokens
-    const int rows = min(kMaxTile, n - c * kMaxTile);
-    for (int i = threadIdx.x; i < rows * p.half; i += kThreads) {
-      const int r = i / p.half;
-      cs[i] = turn_of(p, pos0 + c * kMaxTile + r, i - r * p.half);
+  // Angles of a chunk's tokens, one token's behind the other: element e of pair j at e half / V + j, and `pairs` places between
+  // tokens, so that the lanes of a warp (pairs of one to eight tokens) find theirs in different banks.
+  const int turned_pairs = p.half / V, token_turns = p.half + pairs;
+  auto table = [&](int c) {
+    const int rows = min(p.chunk, n - c * p.chunk);
+    for (int i = threadIdx.x; i < rows * p.half; i += kFp8Threads) {
+      const int r = i / p.half, x = i - r * p.half;
+      cs[r * token_turns + x % V * turned_pairs + x / V] = turn_of(p, pos0 + c * p.chunk + r, x);
+    }
+  };
+  // a head's rows of a chunk, dense, on their way into this warp's part of shared memory
+  T* const mine = reinterpret_cast<T*>(reinterpret_cast<uint8_t*>(cs + p.chunk * token_turns) + warp * (p.chunk * p.dim * sizeof(T)));
+  auto fetch = [&](int job, int h0, int c) {
+    const int rows = min(p.chunk, n - c * p.chunk), h = h0 + (job >> 1);
+    const int64_t stride = (job & 1) == 0 ? p.k_stride : p.v_stride;
+    const T* src = static_cast<const T*>((job & 1) == 0 ? p.k : p.v) + (t0 + c * p.chunk) * stride + static_cast<int64_t>(h) * p.dim;
+    if (V > 1) {
+      const int per_row = p.dim / V;
+      for (int i = lane; i < rows * per_row; i += 32) {
+        const int r = i / per_row;
+        const T* from = src + r * stride + (i - r * per_row) * V;
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(mine + i * V)), "l"(from) : "memory");
+      }
+    } else {
+      for (int i = lane; i < rows * p.dim; i += 32) {
+        const int r = i / p.dim;
+        mine[i] = src[r * stride + (i - r * p.dim)];
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  // pair j of row r, turned where it is to be
+  auto pair_at = [&](int r, int j, bool is_k, PairOf* pr, float (&x0)[V], float (&x1)[V]) {
+    *pr = pair_of<V>(p, j);
+    const Vec<T, V>* row = reinterpret_cast<const Vec<T, V>*>(mine + r * p.dim);
+    widen<T, V>(row[pr->a], x0);
+    widen<T, V>(row[pr->b], x1);
+    if (is_k && pr->turned) {
+      float2 t[V];
+#pragma unroll
+      for (int e = 0; e < V; ++e) t[e] = cs[r * token_turns + e * turned_pairs + j];
+      turn<V>(t, x0, x1);
     }
   };
   // (rounds of 64 heads, so that the maxima have a place whatever the number of heads)
@@ -313,61 +397,50 @@ __device__ __forceinline__ void block_role(const AppendParams& p, int64_t item, 
     const int jobs = 2 * min(64, p.kv_heads - h0);
     for (int step = 0; step < (chunks == 1 ? 1 : 2 * chunks); ++step) {
       const bool measure = step < chunks, store = chunks == 1 || step >= chunks;
-      const int c = store && chunks > 1 ? step - chunks : step;
-      const int rows = min(kMaxTile, n - c * kMaxTile), total = rows << p.pairs_log2;
-      const int64_t tc = t0 + c * kMaxTile;
-      if (step > 0 || h0 > 0) __syncthreads();
+      const int c = step < chunks ? step : step - chunks;
+      const int rows = min(p.chunk, n - c * p.chunk), total = rows << p.pairs_log2;
+      const int64_t tc = t0 + c * p.chunk;
+      __syncwarp();   // every lane is done with this warp's rows before
+      if (warp < jobs) fetch(warp, h0, c);
+      if (step > 0 || h0 > 0) __syncthreads();   // everybody is done with the table before
       table(c);
       __syncthreads();
-      for (int job = warp; job < jobs; job += kWarps) {
+      for (int job = warp; job < jobs; job += kFp8Warps) {
         const bool is_k = (job & 1) == 0;
         const int hr = job >> 1, h = h0 + hr;
-        const T* src = is_k ? static_cast<const T*>(p.k) + tc * p.k_stride : static_cast<const T*>(p.v) + tc * p.v_stride;
-        const int64_t stride = is_k ? p.k_stride : p.v_stride;
-        src += static_cast<int64_t>(h) * p.dim;
-        Vec<T, V> a[kItems], bb[kItems];
-        auto load = [&](int base) {
-#pragma unroll
-          for (int i = 0; i < kItems; ++i) {
-            const int it = base + i * 32 + lane;
-            if (it < total) {
-              const PairOf pr = pair_of<V>(p, it & mask);
-              const Vec<T, V>* s = reinterpret_cast<const Vec<T, V>*>(src + (it >> p.pairs_log2) * stride);
-              a[i] = s[pr.a];
-              bb[i] = s[pr.b];
-            }
-          }
-        };
-        load(0);
         float* scales = is_k ? p.k_scales : p.v_scales;
         const int64_t at = blk * p.kv_heads + h;
         const float old = off > 0 && row0 >= 0 ? scales[at] : 0.0f;
+        if (job != warp) {
+          __syncwarp();
+          fetch(job, h0, c);
+        }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        __syncwarp();
         float amax = 0.0f;
         if (measure) {
-          for (int base = 0; base < total; base += 32 * kItems) {
-            if (base > 0) load(base);
+          // (NaN sets no scale: fmaxf drops it.  Nor does an infinity: then the finite values are gone through by themselves)
+          for (bool finite_only = false;; finite_only = true) {
+            amax = 0.0f;
+            for (int it = lane; it < total; it += 32) {
+              PairOf pr;
+              float x0[V], x1[V];
+              pair_at(it >> p.pairs_log2, it & mask, is_k, &pr, x0, x1);
 #pragma unroll
-            for (int i = 0; i < kItems; ++i) {
-              const int it = base + i * 32 + lane;
-              if (it < total) {
-                const PairOf pr = pair_of<V>(p, it & mask);
-                float x0[V], x1[V];
-                turn<T, V>(a[i], bb[i], is_k && pr.turned, cs + (it >> p.pairs_log2) * p.half, it & mask, x0, x1);
-#pragma unroll
-                for (int e = 0; e < V; ++e) {   // (neither NaN nor an infinity sets a scale)
-                  const float f0 = fabsf(x0[e]), f1 = fabsf(x1[e]);
-                  amax = fmaxf(amax, fmaxf(f0 < INFINITY ? f0 : 0.0f, f1 < INFINITY ? f1 : 0.0f));
-                }
+              for (int e = 0; e < V; ++e) {
+                const float f0 = fabsf(x0[e]), f1 = fabsf(x1[e]);
+                if (!finite_only || f0 < INFINITY) amax = fmaxf(amax, f0);
+                if (!finite_only || f1 < INFINITY) amax = fmaxf(amax, f1);
               }
             }
-          }
 #pragma unroll
-          for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, o));
+            for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, o));
+            if (finite_only || amax < INFINITY) break;
+          }
           if (chunks > 1) {
             if (lane == 0) amax_of[is_k ? 0 : 1][hr] = step == 0 ? amax : fmaxf(amax_of[is_k ? 0 : 1][hr], amax);
             __syncwarp();
           }
-          if (total > 32 * kItems && store) load(0);
         }
         if (!store) continue;
         if (chunks > 1) amax = amax_of[is_k ? 0 : 1][hr];
@@ -383,10 +456,11 @@ __device__ __forceinline__ void block_role(const AppendParams& p, int64_t item, 
             for (int it = lane; it < off * per_row; it += 32) {
               const int r = it / per_row;
               Bytes<W>* d = reinterpret_cast<Bytes<W>*>(head - (r + 1) * row_bytes) + (it - r * per_row);
-              Bytes<W> y = *d;
+              const Bytes<W> y = *d;
+              float x[W];
 #pragma unroll
-              for (int e = 0; e < W; ++e) y.e[e] = quantised(value_of(y.e[e]), ratio);
-              *d = y;
+              for (int e = 0; e < W; ++e) x[e] = value_of(y.e[e]);
+              *d = quantised<W>(x, ratio);
             }
           }
           if (off == 0 || scale > old) {
@@ -394,33 +468,21 @@ __device__ __forceinline__ void block_role(const AppendParams& p, int64_t item, 
             if (lane == 0) scales[at] = scale;
           }
         }
-        for (int base = 0; base < total; base += 32 * kItems) {
-          if (base > 0) load(base);
-#pragma unroll
-          for (int i = 0; i < kItems; ++i) {
-            const int it = base + i * 32 + lane;
-            if (it >= total) continue;
-            const int r = it >> p.pairs_log2, i2 = it & mask;
-            const PairOf pr = pair_of<V>(p, i2);
-            float x0[V], x1[V];
-            turn<T, V>(a[i], bb[i], is_k && pr.turned, cs + r * p.half, i2, x0, x1);
-            if (row0 >= 0) {
-              Bytes<V> y0, y1;
-#pragma unroll
-              for (int e = 0; e < V; ++e) {
-                y0.e[e] = quantised(x0[e], inv);
-                y1.e[e] = quantised(x1[e], inv);
-              }
-              Bytes<V>* d = reinterpret_cast<Bytes<V>*>(head + (c * kMaxTile + r) * row_bytes);
-              d[pr.a] = y0;
-              d[pr.b] = y1;
-            }
-            if (is_k && p.k_out) {
-              Vec<T, V>* d = reinterpret_cast<Vec<T, V>*>(static_cast<T*>(p.k_out) + (tc + r) * p.k_out_stride +
-                                                          static_cast<int64_t>(h) * p.dim);
-              d[pr.a] = narrow<T, V>(x0);
-              d[pr.b] = narrow<T, V>(x1);
-            }
+        for (int it = lane; it < total; it += 32) {
+          const int r = it >> p.pairs_log2;
+          PairOf pr;
+          float x0[V], x1[V];
+          pair_at(r, it & mask, is_k, &pr, x0, x1);
+          if (row0 >= 0) {
+            Bytes<V>* d = reinterpret_cast<Bytes<V>*>(head + (c * p.chunk + r) * row_bytes);
+            d[pr.a] = quantised<V>(x0, inv);
+            d[pr.b] = quantised<V>(x1, inv);
+          }
+          if (is_k && p.k_out) {
+            Vec<T, V>* d = reinterpret_cast<Vec<T, V>*>(static_cast<T*>(p.k_out) + (tc + r) * p.k_out_stride +
+                                                        static_cast<int64_t>(h) * p.dim);
+            d[pr.a] = narrow<T, V>(x0);
+            d[pr.b] = narrow<T, V>(x1);
           }
         }
       }
@@ -429,32 +491,48 @@ __device__ __forceinline__ void block_role(const AppendParams& p, int64_t item, 
 }
 
 template <typename T, int V>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kFp8Threads, 4)
 append_fp8_kernel(const __grid_constant__ AppendParams p) {
-  extern __shared__ float2 cs[];
-  if (static_cast<int64_t>(blockIdx.x) < p.kv_ctas) block_role<T, V>(p, blockIdx.x, cs);
-  else token_role<T, V, false>(p, static_cast<int64_t>(blockIdx.x) - p.kv_ctas, cs);
+  extern __shared__ __align__(16) uint8_t smem[];
+  float2* cs = reinterpret_cast<float2*>(smem);
+  const int warp = threadIdx.x >> 5;
+  // (the blocks first: their chain of waits is the longer one; CTAs of the two kinds alternating were 2 to 10 % slower)
+  if (blockIdx.x < p.kv_ctas) block_role<T, V>(p, blockIdx.x, cs);
+  else token_role<T, V, false>(p, static_cast<int64_t>(blockIdx.x - p.kv_ctas) * kFp8Warps + warp, cs + warp * p.half);
 }
 
 template <typename T, int V>
 int launch_tv(AppendParams p, bool fp8, cudaStream_t stream) {
   p.pairs_log2 = 0;
   while ((2 * V) << p.pairs_log2 < p.dim) ++p.pairs_log2;
-  const int items = (p.heads + (fp8 ? 0 : 2 * p.kv_heads)) << p.pairs_log2;
-  // as many tokens as give every thread its items
-  p.tile = kItems * kThreads / items;
-  p.tile = p.tile < 1 ? 1 : (p.tile > kMaxTile ? kMaxTile : p.tile);
-  int64_t ctas = (p.tokens + p.tile - 1) / p.tile;
+  // few tokens: as many warps for each as fill the GPU, with a pass of 32 pairs or more for every one of them
+  const int64_t passes = (((static_cast<int64_t>(p.heads) + (fp8 ? 0 : 2 * p.kv_heads)) << p.pairs_log2) + 31) / 32;
+  const int64_t parts = kWarpsWanted / p.tokens;
+  p.parts = static_cast<int>(parts < 1 ? 1 : (parts > passes ? passes : parts));
+  const int warps = fp8 ? kFp8Warps : kWarps;
+  int64_t ctas = (p.tokens * p.parts + warps - 1) / warps;
+  size_t smem = static_cast<size_t>(warps) * p.half * sizeof(float2);
   if (fp8) {
     const int64_t kv = p.cu ? p.tokens / p.block_size + 2 * static_cast<int64_t>(p.batch) : p.tokens;
     if (kv > 0x3FFFFFFF) return INFEROP_ERR_LIMIT;
-    p.kv_ctas = static_cast<int>(kv);
+    p.kv_ctas = static_cast<uint32_t>(kv);
     ctas += kv;
+    const int row = p.dim * static_cast<int>(sizeof(T));
+    p.chunk = kMaxJobBytes / row < kMaxTile ? kMaxJobBytes / row : kMaxTile;
+    const size_t need = static_cast<size_t>(p.chunk) * ((p.half + (1 << p.pairs_log2)) * sizeof(float2) + kFp8Warps * row);
+    smem = need > smem ? need : smem;
+    static bool attr_done[64] = {};
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (smem > 48 * 1024 && dev >= 0 && dev < 64 && !attr_done[dev]) {
+      const cudaError_t e = cudaFuncSetAttribute(append_fp8_kernel<T, V>, cudaFuncAttributeMaxDynamicSharedMemorySize, 100 * 1024);
+      if (e != cudaSuccess) return note_cuda_error(e);
+      attr_done[dev] = true;
+    }
   }
   if (ctas > 0x7FFFFFFF) return INFEROP_ERR_LIMIT;
-  const size_t smem = static_cast<size_t>(fp8 ? kMaxTile : p.tile) * p.half * sizeof(float2);   // 16 KB at most
   const unsigned grid = static_cast<unsigned>(ctas);
-  if (fp8) append_fp8_kernel<T, V><<<grid, kThreads, smem, stream>>>(p);
+  if (fp8) append_fp8_kernel<T, V><<<grid, kFp8Threads, smem, stream>>>(p);
   else append_kernel<T, V><<<grid, kThreads, smem, stream>>>(p);
   return check_launch();
 }
