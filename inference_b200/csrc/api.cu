@@ -698,6 +698,7 @@ static int attn_decode(void* out, const void* q, const void* k_cache, const void
   }
   if (dt < 0 || dt > 2) return INFEROP_ERR_DTYPE;
   if (batch > 65535 || static_cast<int64_t>(max_blocks_per_seq) * block_size > 0x7FFFFF00LL) return INFEROP_ERR_LIMIT;
+  if (fp8 && static_cast<int64_t>(fp8->num_blocks) * block_size > 0x7FFFFF00LL) return INFEROP_ERR_LIMIT;
   if (!out || !q || !k_cache || !v_cache || !block_tables || !seq_lens) return INFEROP_ERR_POINTER;
   if ((reinterpret_cast<uintptr_t>(k_cache) & 15u) || (reinterpret_cast<uintptr_t>(v_cache) & 15u)) {
     return INFEROP_ERR_POINTER;
@@ -715,8 +716,11 @@ static int attn_decode(void* out, const void* q, const void* k_cache, const void
     int* counters = nullptr;
     bool zeroed = false;
     const std::unique_lock<std::mutex> lock = attn_scratch(ctx, s, &aws, &counters, &zeroed);
+    if (fp8)
+      return launch_paged_attn_fp8(ctx, out, q, k_cache, v_cache, *fp8, block_tables, seq_lens, dt, batch, num_heads, num_kv_heads,
+                                   head_dim, block_size, max_blocks_per_seq, scale, mod, aws, counters, !zeroed, s);
     return launch_paged_attn_mma(out, q, k_cache, v_cache, block_tables, seq_lens, dt, batch, num_heads, num_kv_heads, head_dim,
-                                 block_size, max_blocks_per_seq, scale, mod, fp8, ctx->sm_count, aws, counters, !zeroed, s);
+                                 block_size, max_blocks_per_seq, scale, mod, ctx->sm_count, aws, counters, !zeroed, s);
   }
   int splits = paged_attn_splits(ctx->sm_count, batch, num_heads, num_kv_heads, block_size, max_blocks_per_seq);
   void *ws = nullptr, *unused = nullptr;

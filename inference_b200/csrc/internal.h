@@ -209,16 +209,23 @@ int launch_paged_attn_decode(void* out, const void* q, const void* k_cache, cons
                              const int32_t* block_tables, const int32_t* seq_lens, int32_t dt, int batch,
                              int num_heads, int num_kv_heads, int head_dim, int block_size, int max_blocks_per_seq,
                              float scale, const ScoreMod& mod, int splits, float* workspace, cudaStream_t stream);
-// attention_mma.cu : on the tensor cores, fp16 (dt 1) / bf16 (dt 2) caches, which calls
-// paged_attn_on_tensor_cores says, and E4M3 caches (`fp8`, else nullptr; block_size % 16 == 0), every call.  workspace of
+// attention_mma.cu : on the tensor cores, fp16 (dt 1) / bf16 (dt 2) caches; which calls
+// paged_attn_on_tensor_cores says.  workspace of
 // paged_attn_mma_workspace_bytes and AttnSet::kCounters zeroed ints of this launch's own; nullptr: every
 // sequence and head group is one CTA's (slower, needs neither).  pdl: programmatic stream serialisation.
 bool paged_attn_on_tensor_cores(int batch, int num_heads, int num_kv_heads, int head_dim, int64_t tokens);
-size_t paged_attn_mma_workspace_bytes();
+size_t paged_attn_mma_workspace_bytes();   // (enough for attention_fp8.cu as well)
 int launch_paged_attn_mma(void* out, const void* q, const void* k_cache, const void* v_cache, const int32_t* block_tables,
                           const int32_t* seq_lens, int32_t dt, int batch, int num_heads, int num_kv_heads, int head_dim,
-                          int block_size, int max_blocks_per_seq, float scale, const ScoreMod& mod, const Fp8Cache* fp8, int sm_count,
-                          float* workspace, int* counters, bool pdl, cudaStream_t stream);
+                          int block_size, int max_blocks_per_seq, float scale, const ScoreMod& mod, int sm_count, float* workspace,
+                          int* counters, bool pdl, cudaStream_t stream);
+// attention_fp8.cu : E4M3 caches, q and out fp16 (dt 1) / bf16 (dt 2); block_size % 16 == 0, fewer than 2^31 cache rows.
+// workspace, counters and pdl as above.
+size_t paged_attn_fp8_workspace_bytes();
+int launch_paged_attn_fp8(DeviceCtx* ctx, void* out, const void* q, const void* k_cache, const void* v_cache, const Fp8Cache& cache,
+                          const int32_t* block_tables, const int32_t* seq_lens, int32_t dt, int batch, int num_heads, int num_kv_heads,
+                          int head_dim, int block_size, int max_blocks_per_seq, float scale, const ScoreMod& mod, float* workspace,
+                          int* counters, bool pdl, cudaStream_t stream);
 // attention_prefill.cu : attention of packed prompts, fp16 (dt 1) / bf16 (dt 2).  Strides are those of a token, in elements.
 struct PrefillArgs {
   void* out;
@@ -290,5 +297,8 @@ int launch_gemm_decode_fused(DeviceCtx* ctx, float* workspace, int* counters, vo
 int make_tensor_map_2d(CUtensorMap* out, const void* base, int elem_bytes, uint64_t rows,
                        uint64_t cols, uint64_t pitch_bytes, uint32_t box_rows, uint32_t box_cols,
                        bool swizzle128);
+// the same with the swizzle by its width: 128, 64 or 0 (none)
+int make_tensor_map_2d_swizzled(CUtensorMap* out, const void* base, int elem_bytes, uint64_t rows, uint64_t cols,
+                                uint64_t pitch_bytes, uint32_t box_rows, uint32_t box_cols, int swizzle_bytes);
 
 }  // namespace ib200
