@@ -31,13 +31,7 @@ namespace {
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
 constexpr float kUp = 15.0f;           // weights are 2^15 p, in their sum and in the denominator
-#ifndef BAL
-#define BAL 0.1f
-#define S64 3
-#define S128 2
-#define S256 2
-#endif
-constexpr float kBalance = BAL;
+constexpr float kBalance = 0.1f;       // of a unit's time and a part's (UnitList::begin)
 
 template <int D>
 struct FCfg {
@@ -49,7 +43,7 @@ struct FCfg {
   static constexpr int kTileBytes = 16 * kRowBytes;
   static constexpr int kHalfBytes = kTiles * kTileBytes;          // K or V of 16 tokens
   static constexpr int kStageBytes = 2 * kHalves * kHalfBytes;    // K, then V
-  static constexpr int kStages = D == 64 ? S64 : D == 128 ? S128 : S256;
+  static constexpr int kStages = D == 64 ? 3 : 2;
   static constexpr int kRec = D + 2;
   static constexpr int kRingBytes = kWarps * kStages * kStageBytes;
   static constexpr int kMetaBytes = kWarps * kStages * kHalves * 8;   // the scales of a step's blocks
@@ -99,15 +93,13 @@ __device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t low_half) {
   return r;
 }
 __device__ __forceinline__ void mma_f16_add(float (&c)[4], uint32_t a0, uint32_t a2, uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %5}, {%7, %8}, {%0, %1, %2, %3};"
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %5}, {%7, %8}, {%0, %1, %2, %3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(0u), "r"(a2), "r"(b0), "r"(b1));
 }
 // (the product alone)
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
 }
@@ -363,21 +355,27 @@ paged_attn_fp8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
             fence_proxy_async_smem();   // the slot's next tiles come by TMA
             __syncwarp();
           }
+          float sc[kHalves][2][4] = {};
+#pragma unroll
+          for (int kk = 0; kk < D / 16; kk += 2) {
+            uint32_t kf[kHalves][4];   // chunks kk and kk + 1 of tile 0's tokens, of tile 1's
+#pragma unroll
+            for (int h = 0; h < kHalves; ++h) ldsm4(at + h * C::kHalfBytes + chunk_place<D>(k_place, kk), kf[h]);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+#pragma unroll
+              for (int i = 0; i < 2 * kHalves; ++i) {   // (the chains of sums alternate)
+                const uint32_t w = kf[i >> 1][2 * (i & 1) + e];
+                mma_f16_add(sc[i >> 1][i & 1], qa[kk + e][0], qa[kk + e][1], e4m3x2_to_f16x2(w & 0xFFFFu), e4m3x2_to_f16x2(w >> 16));
+              }
+            }
+          }
           float s[4 * kHalves];   // tokens 4 quad .. + 3 of either half
 #pragma unroll
           for (int h = 0; h < kHalves; ++h) {
-            float sc[2][4] = {};
-#pragma unroll
-            for (int kk = 0; kk < D / 16; kk += 2) {
-              uint32_t kf[4];   // chunks kk and kk + 1 of tile 0's tokens, of tile 1's
-              ldsm4(at + h * C::kHalfBytes + chunk_place<D>(k_place, kk), kf);
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                mma_f16_add(sc[e >> 1], qa[kk + (e & 1)][0], qa[kk + (e & 1)][1], e4m3x2_to_f16x2(kf[e] & 0xFFFFu), e4m3x2_to_f16x2(kf[e] >> 16));
-            }
             const float f = q_scale * scales[h].x;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) s[4 * h + i] = (swap ? sc[1 - (i >> 1)][i & 1] : sc[i >> 1][i & 1]) * f;
+            for (int i = 0; i < 4; ++i) s[4 * h + i] = (swap ? sc[h][1 - (i >> 1)][i & 1] : sc[h][i >> 1][i & 1]) * f;
           }
           const int behind = len - 1 - (tw + 4 * quad);   // tokens behind this lane's first
           if constexpr (kMod) {

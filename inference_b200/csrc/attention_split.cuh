@@ -227,11 +227,10 @@ __device__ __forceinline__ void finish_pair(const AttnWork& p, float* states, in
   // the sums: a thread's four-element columns side by side, eight loads in flight (sixteen make the stream spill)
   constexpr int kCols = kAttnRows * D / 4 < kThreads ? 1 : kAttnRows * D / 4 / kThreads;
   constexpr int kBatch = 8 / kCols;
-  float4 a[kCols];
+  float4 a[kCols], v[kCols][kBatch];
 #pragma unroll
   for (int j = 0; j < kCols; ++j) a[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  for (int i0 = 0; i0 < parts; i0 += kBatch) {
-    float4 v[kCols][kBatch];
+  auto fetch = [&](float4 (&to)[kCols][kBatch], int i0) {
 #pragma unroll
     for (int j = 0; j < kCols; ++j) {
       const int idx = threadIdx.x + j * kThreads;
@@ -239,10 +238,12 @@ __device__ __forceinline__ void finish_pair(const AttnWork& p, float* states, in
 #pragma unroll
       for (int e = 0; e < kBatch; ++e) {
         asm volatile("ld.global.cg.v4.f32 {%0, %1, %2, %3}, [%4];"
-                     : "=f"(v[j][e].x), "=f"(v[j][e].y), "=f"(v[j][e].z), "=f"(v[j][e].w)
+                     : "=f"(to[j][e].x), "=f"(to[j][e].y), "=f"(to[j][e].z), "=f"(to[j][e].w)
                      : "l"(part(min(i0 + e, parts - 1)) + idx * 4));
       }
     }
+  };
+  auto add = [&](const float4 (&from)[kCols][kBatch], int i0) {
 #pragma unroll
     for (int j = 0; j < kCols; ++j) {
       const int idx = threadIdx.x + j * kThreads;
@@ -252,11 +253,26 @@ __device__ __forceinline__ void finish_pair(const AttnWork& p, float* states, in
       for (int e = 0; e < kBatch; ++e) {
         if (i0 + e >= parts) break;   // (not a weight of zero: the sum may be infinite)
         const float w = wg[i0 + e];
-        a[j].x = fmaf(v[j][e].x, w, a[j].x);
-        a[j].y = fmaf(v[j][e].y, w, a[j].y);
-        a[j].z = fmaf(v[j][e].z, w, a[j].z);
-        a[j].w = fmaf(v[j][e].w, w, a[j].w);
+        a[j].x = fmaf(from[j][e].x, w, a[j].x);
+        a[j].y = fmaf(from[j][e].y, w, a[j].y);
+        a[j].z = fmaf(from[j][e].z, w, a[j].z);
+        a[j].w = fmaf(from[j][e].w, w, a[j].w);
       }
+    }
+  };
+  if constexpr (D == 64) {   // (small states: a second batch is on its way meanwhile)
+    float4 u[kCols][kBatch];
+    fetch(v, 0);
+    for (int i0 = 0; i0 < parts; i0 += 2 * kBatch) {
+      if (i0 + kBatch < parts) fetch(u, i0 + kBatch);
+      add(v, i0);
+      if (i0 + 2 * kBatch < parts) fetch(v, i0 + 2 * kBatch);
+      if (i0 + kBatch < parts) add(u, i0 + kBatch);
+    }
+  } else {
+    for (int i0 = 0; i0 < parts; i0 += kBatch) {
+      fetch(v, i0);
+      add(v, i0);
     }
   }
 #pragma unroll
