@@ -10,13 +10,21 @@
 //   * S = Q K^T and O += P V are tcgen05.mma with accumulators in tensor memory; P goes back into tensor memory, over the
 //     scores that it came from, and is the A operand from there.  A thread has a row of S: neither maximum nor sum
 //     needs a shuffle.
-//   * K and V blocks come through one ring by TMA.  V lies as it is (tokens outside): operand B with N contiguous.
+//   * A V block and the next K block are one stage of a ring that TMA fills: one wait and one release per block for the
+//     warp that issues the MMAs, whose own time between two products is the tensor cores' idle time (535 -> 525 us below).
+//     V lies as it is (tokens outside): operand B with N contiguous.
 //   * O is rescaled only where a row's maximum grew by more than 2^8 since the last time (the exponentials stay below
 //     that), which is rare behind the first blocks; the row's thread does it in tensor memory.
 //   * Rows of a V block behind the prompt's end are set to zero in shared memory: they are another prompt's, and 0 x NaN
 //     would be NaN.  Their scores are masked.
 // P is rounded to the operands' type for the second product: 2^-9 (bf16) or 2^-12 relative per term, of random sign, where
 // the sum is rounded to the same type at the end anyway; row sums are of the unrounded values, in fp32.
+//
+// Bound by the tensor cores and, between a tile's two products, by the chain of its softmax: 8192 tokens, 32 heads over 8 KV
+// heads of 128, bf16, causal: 525 us = 1046 TFLOP/s in long runs; a pair of blocks (256 rows, 128 keys) takes about 3400 cycles, of
+// which the products are 2048 and the softmax of a tile, which the other tile's products run beside, 1850.  Not faster:
+// blocks of 64 keys with two score buffers per tile (products of 64 columns run at half the rate: 640 us), a quarter of the
+// exponentials by polynomials (558), P handed over in halves (546), two threads per row (564), an MMA warp per tile (600).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -35,6 +43,7 @@ constexpr int kTile = 128;                // query rows of a tile: the lanes of 
 // two warpgroups with a row per thread; the issuer of MMAs, the TMA producer and two warps that only give up their registers:
 // 168 per thread at launch, 208 for the first two groups and 88 for the last make the same sum
 constexpr int kThreads = 384;
+constexpr int kSoftmaxWarps = 8;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRescaleAbove = 8.0f;     // powers of two that a maximum may lag behind
 
@@ -44,8 +53,9 @@ struct PCfg {
   static constexpr int kBlock = D == 256 ? 64 : 128;              // keys of a block
   static constexpr int kBoxes = D / 64;                           // 128-byte columns of a row
   static constexpr int kQBytes = kTile * D * 2;                   // of one tile
-  static constexpr int kStageBytes = kBlock * D * 2;              // a K or V block
-  static constexpr int kStages = D == 64 ? 6 : 4;
+  static constexpr int kBlockBytes = kBlock * D * 2;              // of K or V
+  static constexpr int kStageBytes = 2 * kBlockBytes;             // V of a block, then K of the next
+  static constexpr int kStages = D == 64 ? 3 : 2;
   static constexpr int kBarOffset = kTiles * kQBytes + kStages * kStageBytes;
   static constexpr int kSmemBytes = kBarOffset + 256 + 1024;      // (the base is rounded up to 1024)
   // tensor memory: two score buffers (one per tile, or of alternate blocks), then the tiles' sums
@@ -116,6 +126,84 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volati
   return __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity, abort_flag, status, site));
 }
 
+// A row's products of a block -> its scores in base 2: capped, less the distance bias.  ahead: the row's position from the
+// block's first key; behind: no key that counts lies behind the row.
+// tanh: where every score of the warp is within the cap, an odd polynomial of degree 11 (off by 2.4e-7 on [-1, 1], least maximum of
+// the error) on the FMA units; else 1 - 2 / (1 + e^2x), whose two special functions are the bound of the kernel then (8192
+// tokens, 32 heads of 128: 1640 us against 750).
+template <int kChunks>
+__device__ __forceinline__ void change_scores(uint32_t (&s)[kChunks][32], const PrefillParams& p, float slope, int ahead, bool behind) {
+  const auto twice = [](float v) { return make_float2(v, v); };
+  const float2 f2 = twice(p.scale_log2e);
+  if (p.cap_log2e > 0.0f) {
+    float top = 0.0f;
+#pragma unroll
+    for (int c = 0; c < kChunks; ++c) {
+#pragma unroll
+      for (int e = 0; e < 32; ++e) top = fmaxf(top, fabsf(__uint_as_float(s[c][e])));
+    }
+    if (__all_sync(0xFFFFFFFFu, top * fabsf(p.scale_log2e) <= 1.0f)) {   // (NaN is no hindrance: it stays NaN)
+      const float2 cap2 = twice(p.cap_log2e);
+#pragma unroll
+      for (int c = 0; c < kChunks; ++c) {
+#pragma unroll
+        for (int e = 0; e < 32; e += 2) {
+          const float2 y = __fmul2_rn(make_float2(__uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1])), f2), z = __fmul2_rn(y, y);
+          float2 t = __ffma2_rn(twice(-0.00283946399576962f), z, twice(0.01611417718231678f));
+          t = __ffma2_rn(t, z, twice(-0.05097286030650139f));
+          t = __ffma2_rn(t, z, twice(0.13253524899482727f));
+          t = __ffma2_rn(t, z, twice(-0.3332400321960449f));
+          t = __ffma2_rn(t, z, twice(0.9999968409538269f));
+          t = __fmul2_rn(t, __fmul2_rn(y, cap2));
+          s[c][e] = __float_as_uint(t.x);
+          s[c][e + 1] = __float_as_uint(t.y);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int c = 0; c < kChunks; ++c) {
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+          float r;
+          asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + ex2(__uint_as_float(s[c][e]) * p.scale_log2e * (2.0f * kLog2e))));
+          s[c][e] = __float_as_uint(p.cap_log2e * fmaf(-2.0f, r, 1.0f));
+        }
+      }
+    }
+  } else {
+#pragma unroll
+    for (int c = 0; c < kChunks; ++c) {
+#pragma unroll
+      for (int e = 0; e < 32; e += 2) {
+        const float2 y = __fmul2_rn(make_float2(__uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1])), f2);
+        s[c][e] = __float_as_uint(y.x);
+        s[c][e + 1] = __float_as_uint(y.y);
+      }
+    }
+  }
+  if (p.slopes == nullptr) return;
+  if (behind) {
+    float2 d = make_float2(static_cast<float>(-ahead), static_cast<float>(1 - ahead));   // minus the distance
+#pragma unroll
+    for (int c = 0; c < kChunks; ++c) {
+#pragma unroll
+      for (int e = 0; e < 32; e += 2) {
+        const float2 y = __ffma2_rn(twice(slope), d, make_float2(__uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1])));
+        s[c][e] = __float_as_uint(y.x);
+        s[c][e + 1] = __float_as_uint(y.y);
+        d = __fadd2_rn(d, twice(2.0f));   // (whole numbers)
+      }
+    }
+  } else {
+#pragma unroll
+    for (int c = 0; c < kChunks; ++c) {
+#pragma unroll
+      for (int e = 0; e < 32; ++e)
+        s[c][e] = __float_as_uint(fmaf(-slope, fabsf(static_cast<float>(ahead - c * 32 - e)), __uint_as_float(s[c][e])));
+    }
+  }
+}
+
 // where a CTA's tile i lies
 struct TileAt {
   int head, q0, blocks;
@@ -184,7 +272,7 @@ prefill_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     tma_prefetch_desc(&map_k);
     tma_prefetch_desc(&map_v);
   }
-  if (warp == 8) {
+  if (warp == kSoftmaxWarps) {
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
@@ -193,9 +281,9 @@ prefill_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
   tc_fence_after_sync();
   const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, *tmem_slot, 0);
 
-  if (warp >= 8) {
+  if (warp >= kSoftmaxWarps) {
     reg_dealloc<88>();
-    if (warp == 9) {
+    if (warp == kSoftmaxWarps + 1) {
       // ------------------------------ TMA producer ------------------------
       bool ok = true;
       if (!p.no_loads) {
@@ -209,20 +297,20 @@ prefill_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         }
         int stage = 0;
         uint32_t phase = 0;
-        for (int it = 0; it < 2 * blocks; ++it) {           // K 0, V 0, K 1, V 1, ...
-          const int j = it >> 1;
-          const bool is_v = (it & 1) != 0;
+        for (int j = -1; j < blocks; ++j) {                // K 0 alone, then V j with K j + 1
           if (!warp_wait(&empty[stage], phase ^ 1u, abort_flag, p.status, kSiteAProducerEmpty)) {
             ok = false;
             break;
           }
           uint8_t* dst = ring + stage * C::kStageBytes;
-          const bool tail = is_v && (j + 1) * BN > n;        // (once, in the last block of the prompt)
+          const bool v = j >= 0, k = j + 1 < blocks;
+          const bool tail = v && (j + 1) * BN > n;         // (once, in the last block of the prompt: there is no K behind it)
           uint64_t* bar = tail ? edge : &full[stage];
           if (lane == 0) {
-            mbar_arrive_expect_tx(bar, C::kStageBytes);
-            for (int x = 0; x < C::kBoxes; ++x)
-              tma_load_2d(dst + x * (BN * 128), is_v ? &map_v : &map_k, bar, kv_col + x * 64, c0 + j * BN);
+            mbar_arrive_expect_tx(bar, (v ? C::kBlockBytes : 0) + (k ? C::kBlockBytes : 0));
+            for (int x = 0; k && x < C::kBoxes; ++x)
+              tma_load_2d(dst + C::kBlockBytes + x * (BN * 128), &map_k, bar, kv_col + x * 64, c0 + (j + 1) * BN);
+            for (int x = 0; v && x < C::kBoxes; ++x) tma_load_2d(dst + x * (BN * 128), &map_v, bar, kv_col + x * 64, c0 + j * BN);
           }
           __syncwarp();
           if (tail) {
@@ -250,25 +338,22 @@ prefill_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         while (clock64() - w0 < (1LL << 22)) {
         }
       }
-    } else if (warp == 8) {
+    } else if (warp == kSoftmaxWarps) {
       // ------------------------------ MMA issuer --------------------------
       constexpr uint32_t idesc_s = umma_idesc_16bit_f32(Num<T>::kFormat, kTile, BN, false);
       constexpr uint32_t idesc_o = umma_idesc_16bit_f32(Num<T>::kFormat, kTile, D, true);
       const uint32_t q_addr = smem_u32(smem), ring_addr = smem_u32(ring);
-      // K block j is element 2 j of the ring's sequence, V block j element 2 j + 1
-      auto stage_of = [&](int it) { return it % C::kStages; };
-      auto wait_full = [&](int it) {
-        return warp_wait(&full[stage_of(it)], (it / C::kStages) & 1, abort_flag, p.status, kSiteAMmaFull);
-      };
+      int stage = 0;
+      uint32_t phase = 0;
       auto scores = [&](int i, int j) {       // S = Q_i K_j^T
         const uint32_t d = tmem + C::kSCol + (NT == 2 ? i : j & 1) * BN;
-        const uint32_t k = ring_addr + stage_of(2 * j) * C::kStageBytes, q = q_addr + i * C::kQBytes;
+        const uint32_t k = ring_addr + stage * C::kStageBytes + C::kBlockBytes, q = q_addr + i * C::kQBytes;
         if (elect_one()) {
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk) {
             const uint32_t in_box = (kk % 4) * 32;
-            umma_16bit_ss(d, umma_desc_k_sw128(q + (kk / 4) * (kTile * 128) + in_box), umma_desc_k_sw128(k + (kk / 4) * (BN * 128) + in_box),
-                          idesc_s, kk > 0 ? 1u : 0u);
+            umma_16bit_ss(d, umma_desc_k_sw128(q + (kk / 4) * (kTile * 128) + in_box),
+                          umma_desc_k_sw128(k + (kk / 4) * (BN * 128) + in_box), idesc_s, kk > 0 ? 1u : 0u);
           }
           umma_commit(&s_full[NT == 2 ? i : j & 1]);
         }
@@ -276,57 +361,40 @@ prefill_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
       };
       auto sums = [&](int i, int j) {         // O_i += P V_j
         const uint32_t a = tmem + C::kSCol + (NT == 2 ? i : j & 1) * BN;
-        const uint32_t v = ring_addr + stage_of(2 * j + 1) * C::kStageBytes;
+        const uint32_t v = ring_addr + stage * C::kStageBytes;
         if (elect_one()) {
 #pragma unroll
           for (int kk = 0; kk < BN / 16; ++kk)
-            umma_16bit_ts(tmem + C::kOCol + i * D, a + kk * 8, umma_desc_mn_sw128(v + kk * 2048, BN * 128), idesc_o, j > 0 || kk > 0 ? 1u : 0u);
+            umma_16bit_ts(tmem + C::kOCol + i * D, a + kk * 8, umma_desc_mn_sw128(v + kk * 2048, BN * 128), idesc_o,
+                          j > 0 || kk > 0 ? 1u : 0u);
           umma_commit(&o_done[i]);
         }
         __syncwarp();
       };
-      auto release = [&](int it) {
-        if (elect_one()) umma_commit(&empty[stage_of(it)]);
-        __syncwarp();
-      };
-      auto wait_p = [&](int i, int j) {
-        return warp_wait(&p_full[NT == 2 ? i : j & 1], (NT == 2 ? j : j >> 1) & 1, abort_flag, p.status, kSiteAMmaP);
-      };
       const int tile_blocks[2] = {t0.blocks, t1.blocks};
-      bool ok = warp_wait(q_full, 0u, abort_flag, p.status, kSiteAMmaQ) && wait_full(0);
-      if (ok) {
+      bool ok = warp_wait(q_full, 0u, abort_flag, p.status, kSiteAMmaQ);
+      // MMAs run in the order of their issue: a score buffer is written again behind the product that reads its P.  One tile per
+      // CTA: the scores of the next block are there before P is waited for.
+      for (int j = -1; ok && j < blocks; ++j) {
+        ok = warp_wait(&full[stage], phase, abort_flag, p.status, kSiteAMmaFull);
+        if (!ok) break;
         tc_fence_after_sync();
-#pragma unroll
-        for (int i = 0; i < NT; ++i)
-          if (tile_blocks[i] > 0) scores(i, 0);
-        release(0);
-      }
-      for (int j = 0; ok && j < blocks; ++j) {
-        if (NT == 1 && j + 1 < blocks) {
-          ok = wait_full(2 * j + 2);
-          if (!ok) break;
-          tc_fence_after_sync();
-          scores(0, j + 1);
-          release(2 * j + 2);
-        }
-        ok = wait_full(2 * j + 1);
+        if (NT == 1 && j + 1 < blocks) scores(0, j + 1);
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
-          if (!ok) break;
-          if (j < tile_blocks[i]) {
-            ok = wait_p(i, j);
+          if (j >= 0 && j < tile_blocks[i]) {
+            ok = ok && warp_wait(&p_full[NT == 2 ? i : j & 1], (NT == 2 ? j : j >> 1) & 1, abort_flag, p.status, kSiteAMmaP);
             if (!ok) break;
             tc_fence_after_sync();
             sums(i, j);
           }
-          if (i == NT - 1) release(2 * j + 1);
-          if (NT == 2 && j + 1 < blocks) {
-            if (i == 0) ok = wait_full(2 * j + 2);
-            if (!ok) break;
-            tc_fence_after_sync();
-            if (j + 1 < tile_blocks[i]) scores(i, j + 1);
-            if (i == 1) release(2 * j + 2);
-          }
+          if (NT == 2 && j + 1 < tile_blocks[i]) scores(i, j + 1);
+        }
+        if (elect_one()) umma_commit(&empty[stage]);
+        __syncwarp();
+        if (++stage == C::kStages) {
+          stage = 0;
+          phase ^= 1u;
         }
       }
     }
@@ -338,7 +406,7 @@ prefill_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
       const TileAt t = i == 0 ? t0 : t1;
       const int pos = t.q0 + (warp & 3) * 32 + lane;
       const int lim = min(n, max(pos + 1, prefix));          // keys from here on are masked (rows behind the prompt: any)
-      const int lim_warp = __shfl_sync(0xFFFFFFFFu, lim, 0);
+      const int lim_warp = __shfl_sync(0xFFFFFFFFu, lim, 0), pos_warp = __shfl_sync(0xFFFFFFFFu, pos, 0);
       const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
       const uint32_t o_at = tmem + lanes + C::kOCol + i * D;
       const float slope = kMod && p.slopes ? __ldg(p.slopes + t.head) * kLog2e : 0.0f;
@@ -356,22 +424,7 @@ prefill_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         tmem_ld_wait();
 #pragma unroll
         for (int c = 0; c < BN / 32; ++c) pin32(s[c]);
-        if constexpr (kMod) {
-#pragma unroll
-          for (int c = 0; c < BN / 32; ++c) {
-#pragma unroll
-            for (int e = 0; e < 32; ++e) {
-              float x = __uint_as_float(s[c][e]) * p.scale_log2e;
-              if (p.cap_log2e > 0.0f) {
-                // tanh(x) = 1 - 2 / (1 + e^2x): off by some 2^-22, which the cap multiplies
-                float r;
-                asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + ex2(x * (2.0f * kLog2e))));
-                x = p.cap_log2e * fmaf(-2.0f, r, 1.0f);
-              }
-              s[c][e] = __float_as_uint(fmaf(-slope, fabsf(static_cast<float>(pos - (j * BN + c * 32 + e))), x));
-            }
-          }
-        }
+        if constexpr (kMod) change_scores<BN / 32>(s, p, slope, pos - j * BN, (j + 1) * BN <= pos_warp + 1 || prefix == 0);
         if ((j + 1) * BN > lim_warp) {
 #pragma unroll
           for (int c = 0; c < BN / 32; ++c) {
@@ -468,7 +521,7 @@ prefill_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
-  if (warp == 8) tmem_dealloc(tmem, 512);
+  if (warp == kSoftmaxWarps) tmem_dealloc(tmem, 512);
 }
 
 template <typename T, int D, bool kMod>
