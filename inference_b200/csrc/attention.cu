@@ -26,6 +26,7 @@
 #include <math.h>
 #include <stdint.h>
 
+#include "attention_split.cuh"
 #include "internal.h"
 
 namespace ib200 {
@@ -153,11 +154,11 @@ paged_attn_kernel(const AttnParams p) {
 #pragma unroll
     for (int e = 0; e < C::EPL; ++e) qf[g][e] = to_f32<T>(qrow[elem_index<C>(sub, e)]) * p.scale_log2e;
   }
-  float slope[kMod ? GT : 1];
-  if constexpr (kMod) {
-#pragma unroll
-    for (int g = 0; g < GT; ++g) slope[g] = p.slopes ? __ldg(p.slopes + head0 + g) * 1.4426950408889634f : 0.0f;
-  }
+  // kMod: the scores that this lane owns between the reduction and the hand-out below are of one head
+  constexpr int kOwned = GT * kBatch >= C::LPT ? GT * kBatch / C::LPT : 1, kShare = GT * kBatch >= C::LPT ? 1 : C::LPT / (GT * kBatch);
+  static_assert(kOwned <= kBatch, "one head");
+  const int first_owned = sub / kShare * kOwned;
+  const float slope = kMod && p.slopes ? __ldg(p.slopes + head0 + first_owned / kBatch) * 1.4426950408889634f : 0.0f;
   float m[GT], l[GT], acc[GT][C::EPL];
 #pragma unroll
   for (int g = 0; g < GT; ++g) {
@@ -269,13 +270,21 @@ paged_attn_kernel(const AttnParams p) {
     {
       constexpr int CF = NV >= C::LPT ? NV / C::LPT : 1;      // totals a lane owns after the butterfly
       constexpr int LF = NV >= C::LPT ? 1 : C::LPT / NV;      // lanes that hold the same total
+      if constexpr (kMod) {
+#pragma unroll
+        for (int i = 0; i < CF; ++i) {
+          const int far = len - 1 - (tb + (first_owned + i) % kBatch * C::NS);
+          if constexpr (sizeof(T) == 4) {   // (the accurate function: fp32 results show its error)
+            if (p.cap_log2e > 0.0f) val[i] = p.cap_log2e * tanhf(val[i]);
+            val[i] = fmaf(-slope, static_cast<float>(far), val[i]);
+          } else {
+            val[i] = scored(val[i], p.cap_log2e, slope, far);
+          }
+        }
+      }
 #pragma unroll
       for (int v = 0; v < NV; ++v) {
-        float tot = __shfl_sync(0xFFFFFFFFu, val[v % CF], (v / CF) * LF, C::LPT);
-        if constexpr (kMod) {
-          if (p.cap_log2e > 0.0f) tot = p.cap_log2e * tanhf(tot);
-          tot = fmaf(-slope[v / kBatch], static_cast<float>(len - 1 - (tb + v % kBatch * C::NS)), tot);
-        }
+        const float tot = __shfl_sync(0xFFFFFFFFu, val[v % CF], (v / CF) * LF, C::LPT);
         s2[v / kBatch][v % kBatch] = valid[v % kBatch] ? tot : -INFINITY;
       }
     }
