@@ -686,7 +686,7 @@ static int kv_append(const KvAppendArgs& a, cudaStream_t s) {
   return launch_kv_append(a, s);
 }
 
-static bool softcap_ok(float cap) { return cap >= 0.0f && cap < INFINITY; }
+static bool softcap_ok(float cap, float scale) { return cap == 0.0f || (cap > 0.0f && cap < INFINITY && fabsf(scale / cap) < INFINITY); }
 
 static int attn_decode(void* out, const void* q, const void* k_cache, const void* v_cache, const Fp8Cache* fp8,
                        const int32_t* block_tables, const int32_t* seq_lens, int32_t dt, int32_t batch, int32_t num_heads,
@@ -781,7 +781,7 @@ int inferop_paged_attn_decode_scored(void* out, const void* q, const void* k_cac
                                      const int32_t* block_tables, const int32_t* seq_lens, int32_t dt, int32_t batch,
                                      int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, int32_t block_size,
                                      int32_t max_blocks_per_seq, float scale, float softcap, const float* alibi_slopes, void* stream) {
-  if (!softcap_ok(softcap)) return INFEROP_ERR_SHAPE;
+  if (!softcap_ok(softcap, scale)) return INFEROP_ERR_SHAPE;
   return attn_decode(out, q, k_cache, v_cache, nullptr, block_tables, seq_lens, dt, batch, num_heads, num_kv_heads, head_dim, block_size,
                      max_blocks_per_seq, scale, ScoreMod{softcap, alibi_slopes}, stream);
 }
@@ -790,7 +790,7 @@ int inferop_paged_attn_decode_fp8(void* out, const void* q, const void* k_cache,
                                   const void* v_scales, const int32_t* block_tables, const int32_t* seq_lens, int32_t dt, int32_t batch,
                                   int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, int32_t block_size, int32_t num_blocks,
                                   int32_t max_blocks_per_seq, float scale, float softcap, const float* alibi_slopes, void* stream) {
-  if (block_size % 16 != 0 || num_blocks <= 0 || !softcap_ok(softcap)) return INFEROP_ERR_SHAPE;
+  if (block_size % 16 != 0 || num_blocks <= 0 || !softcap_ok(softcap, scale)) return INFEROP_ERR_SHAPE;
   if (dt == 0) return INFEROP_ERR_DTYPE;
   if (!k_scales || !v_scales) return INFEROP_ERR_POINTER;
   const Fp8Cache fp8 = {static_cast<const float*>(k_scales), static_cast<const float*>(v_scales), num_blocks};
@@ -803,7 +803,7 @@ int inferop_prefill_attn(void* out, int64_t out_stride, const void* q, int64_t q
                          int64_t tokens, int32_t batch, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, float scale,
                          float softcap, const float* alibi_slopes, void* stream) {
   if (tokens <= 0 || batch <= 0 || num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads != 0 ||
-      (head_dim != 64 && head_dim != 128 && head_dim != 256) || !softcap_ok(softcap)) {
+      (head_dim != 64 && head_dim != 128 && head_dim != 256) || !softcap_ok(softcap, scale)) {
     return INFEROP_ERR_SHAPE;
   }
   const int64_t q_row = static_cast<int64_t>(num_heads) * head_dim, kv_row = static_cast<int64_t>(num_kv_heads) * head_dim;

@@ -3,15 +3,22 @@
 // (attention_split.cuh).
 //
 // The bytes are half of a 16-bit cache's, so what an SM does per row has to be half as much too:
-//   * A warp's step is 16 tokens, which lie inside one cache block (block sizes are multiples of 16): two tiled TMA loads by
-//     one lane, into a ring of the warp's own; the block's scales come along by cp.async, and multiply the step's scores and its sums
-//     once each.
-//   * Both products are fp16 ones, in which E4M3 is exact.  (mma.sync on E4M3 operands is two fp16 products with conversions of both
-//     operands here, and q would need two or three E4M3 parts.)  Weights are p = hi + lo, 22 bits of p 2^15, in rows 0-7 and 8-15
-//     of one product; E4M3 has no infinity that a zero part could meet.
+//   * A warp's step is 32 tokens (16 at head size 256): two cache blocks or two halves of one (block sizes are multiples of 16).
+//     One lane asks for its K and V rows by tiled TMA loads, into a ring of the warp's own; the blocks' scales come along by
+//     cp.async, and multiply a block's scores and its sums once each.
+//   * Both products are fp16 ones, in which E4M3 is exact.  (With E4M3 operands mma.sync counted twice as many products and a
+//     conversion per operand register, and q needs two or three E4M3 parts: 150 us in the place of 133 at the time.)  Weights are
+//     p = hi + lo, 22 bits of p 2^15, in rows 0-7 and 8-15 of one product; E4M3 has no infinity that a zero part could meet.
 //   * A byte of K or V is converted once, straight from ldmatrix: K as it lies, four dims of a token in a register; V transposed
 //     by bytes, four tokens of a dim.  The dims of q and the tokens of a score tile are ordered so that a register's halves
 //     are the two halves of an operand, and a thread's four scores belong to the four tokens that it holds of V.
+//
+// Bound by instruction latency with twelve warps on an SM, as many as 168 registers allow: 387 instructions per 16 tokens (590 in
+// the form of attention_mma.cu with rows copied by cp.async), 44 % of the issue slots.  Measured (bf16, 32 heads over 8 KV
+// heads of 128, blocks of 16 in random order): 64 x 4096 tokens 120 us = 4.5 TB/s (133 us in that form; 173 us
+// over a bf16 cache), 64 x 1000 43 us, one sequence of 777 10.8 us (15); 16 heads over 8 of 256, 64 x 4096: 220 us = 4.9 TB/s; one
+// sequence of 65536, 8 heads over one of 64: 21 us.  A producer warp for all tiles was slower (250 us: its chain of loads
+// is as long as a unit), and so were eight warps per CTA (150 us: 128 registers, spills).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -57,7 +64,7 @@ struct FCfg {
   static constexpr bool fits(int gt) { return ctas_per_sm(gt) * (smem_bytes(gt) + 1280) <= 233472 && smem_bytes(gt) + 256 <= 232448; }
   static_assert(fits(4) && fits(kAttnRows), "resident CTAs");
   static_assert(kAttnSms * 3 <= AttnSet::kCounters, "a counter per CTA");
-  static constexpr size_t kWorkspaceBytes = static_cast<size_t>(kAttnSms) * 3 * 2 * kAttnRows * kRec * sizeof(float);
+  static constexpr size_t kWorkspaceBytes = static_cast<size_t>(kAttnSms) * kRegCtas * 2 * kAttnRows * kRec * sizeof(float);
 };
 
 struct Fp8AttnParams : AttnWork {
@@ -72,6 +79,7 @@ struct Fp8AttnParams : AttnWork {
   float scale_log2e;       // what a product is multiplied by: to base 2 or, capped, to the cap's units
   float cap_log2e;         // kMod: the cap (0: none), to base 2
   const float* slopes;     // kMod: a head's loss per token of distance, or null
+  int no_loads;            // test hook: no tile is asked for
   DeviceStatus* status;
 };
 
@@ -94,14 +102,14 @@ __device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t low_half) {
 }
 __device__ __forceinline__ void mma_f16_add(float (&c)[4], uint32_t a0, uint32_t a2, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %5}, {%7, %8}, {%0, %1, %2, %3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a0), "r"(0u), "r"(a2), "r"(b0), "r"(b1));
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a0), "r"(0u), "r"(a2), "r"(b0), "r"(b1));
 }
 // (the product alone)
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
-      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+               : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
 }
 __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
@@ -189,7 +197,8 @@ paged_attn_fp8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
   auto lookup = [&]() -> int {
     const int t = pre.t + warp * C::kTok + (lane & (kHalves - 1)) * 16;
     if (pre.left <= 0 || t >= pre.len) return -1;
-    const int blk = __ldg(p.block_tables + static_cast<int64_t>(pre.b) * p.max_blocks + (p.block_shift >= 0 ? t >> p.block_shift : t / p.block_size));
+    const int j = p.block_shift >= 0 ? t >> p.block_shift : t / p.block_size;
+    const int blk = __ldg(p.block_tables + static_cast<int64_t>(pre.b) * p.max_blocks + j);
     return blk < p.num_blocks ? blk : -1;
   };
   int next_block = lookup();
@@ -210,7 +219,7 @@ paged_attn_fp8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
     }
     holes = (holes & ~(((1u << kHalves) - 1u) << (slot * kHalves))) | none << (slot * kHalves);
     if (any) {
-      if (lane == 0) {
+      if (lane == 0 && !p.no_loads) {
         uint8_t* dst = ring + slot * C::kStageBytes;
         const int off = p.block_shift >= 0 ? t & block_mask : t % p.block_size;
         if (kHalves == 2 && p.wide) {
@@ -338,7 +347,10 @@ paged_attn_fp8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
           float2 scales[kHalves];
 #pragma unroll
           for (int h = 0; h < kHalves; ++h)
-            asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(scales[h].x), "=f"(scales[h].y) : "r"(meta + (slot * kHalves + h) * 8) : "memory");
+            asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];"
+                         : "=f"(scales[h].x), "=f"(scales[h].y)
+                         : "r"(meta + (slot * kHalves + h) * 8)
+                         : "memory");
           const bool partial = tw + C::kTok > len || none != 0u;
           if (partial) {
             // rows that are no token's: whatever is there, NaN perhaps, and 0 x NaN would reach the sums
@@ -422,7 +434,8 @@ paged_attn_fp8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
                 float d[4];
-                mma_f16(d, hi[2 * h], lo[2 * h], hi[2 * h + 1], lo[2 * h + 1], e4m3x2_to_f16x2(vf[i] & 0xFFFFu), e4m3x2_to_f16x2(vf[i] >> 16));
+                mma_f16(d, hi[2 * h], lo[2 * h], hi[2 * h + 1], lo[2 * h + 1], e4m3x2_to_f16x2(vf[i] & 0xFFFFu),
+                        e4m3x2_to_f16x2(vf[i] >> 16));
                 add_scaled(acc[2 * c + i], d, v2);
               }
             }
@@ -449,8 +462,9 @@ paged_attn_fp8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
         st[D + 1] = l;
       }
     }
-    finish_pair<kWarps, D, C::kUnit, true>(p, states, p.gt, sh_last, static_cast<T*>(p.out) + (static_cast<int64_t>(b) * p.num_heads + head0) * D,
-                                           len, t_first, t_last, use.left, share, seg_u, [](float v) { return narrow16<T>(v); });
+    T* out = static_cast<T*>(p.out) + (static_cast<int64_t>(b) * p.num_heads + head0) * D;
+    finish_pair<kWarps, D, C::kUnit, true>(p, states, p.gt, sh_last, out, len, t_first, t_last, use.left, share, seg_u,
+                                           [](float v) { return narrow16<T>(v); });
     __syncthreads();   // the states may be overwritten now
   }
   asm volatile("cp.async.wait_group 0;" ::: "memory");
@@ -500,7 +514,8 @@ int launch_d(const CUtensorMap& mk, const CUtensorMap& mv, const Fp8AttnParams& 
 }
 
 template <typename T, bool kMod>
-int launch_t(const CUtensorMap& mk, const CUtensorMap& mv, const Fp8AttnParams& p, int head_dim, int sm_count, bool pdl, cudaStream_t stream) {
+int launch_t(const CUtensorMap& mk, const CUtensorMap& mv, const Fp8AttnParams& p, int head_dim, int sm_count, bool pdl,
+             cudaStream_t stream) {
   switch (head_dim) {
     case 64: return launch_d<T, 64, kMod>(mk, mv, p, sm_count, pdl, stream);
     case 128: return launch_d<T, 128, kMod>(mk, mv, p, sm_count, pdl, stream);
@@ -545,6 +560,7 @@ int launch_paged_attn_fp8(DeviceCtx* ctx, void* out, const void* q, const void* 
   p.scale_log2e = mod.softcap > 0.0f ? scale / mod.softcap : scale * 1.4426950408889634f;
   p.cap_log2e = mod.softcap * 1.4426950408889634f;
   p.slopes = mod.slopes;
+  p.no_loads = options().debug_no_loads;
   p.status = ctx->status;
   // (rows of a KV head are head_dim bytes of a token's num_kv_heads head_dim)
   const uint64_t rows = static_cast<uint64_t>(cache.num_blocks) * block_size, cols = static_cast<uint64_t>(num_kv_heads) * head_dim;
@@ -556,7 +572,9 @@ int launch_paged_attn_fp8(DeviceCtx* ctx, void* out, const void* q, const void* 
   if (rc == INFEROP_OK) rc = make_tensor_map_2d_swizzled(&mv, v_cache, 1, rows, cols, cols, box_rows, box, box);
   if (rc != INFEROP_OK) return rc;
   const int sms = ctx->sm_count;
-  if (dt == 1) return mod.any() ? launch_t<__half, true>(mk, mv, p, head_dim, sms, pdl, stream) : launch_t<__half, false>(mk, mv, p, head_dim, sms, pdl, stream);
+  if (dt == 1)
+    return mod.any() ? launch_t<__half, true>(mk, mv, p, head_dim, sms, pdl, stream)
+                     : launch_t<__half, false>(mk, mv, p, head_dim, sms, pdl, stream);
   return mod.any() ? launch_t<__nv_bfloat16, true>(mk, mv, p, head_dim, sms, pdl, stream)
                    : launch_t<__nv_bfloat16, false>(mk, mv, p, head_dim, sms, pdl, stream);
 }

@@ -394,8 +394,9 @@ paged_attn_mma_kernel(const MmaAttnParams p) {
         st[D + 1] = l;
       }
     }
-    finish_pair<kWarps, D, kUnit, false>(p, states, kRows, sh_last, static_cast<T*>(p.out) + (static_cast<int64_t>(b) * p.num_heads + head0) * D, len,
-                                         t_first, t_last, use.left, share, seg_u, [](float v) { return O::narrow(v); });
+    T* out = static_cast<T*>(p.out) + (static_cast<int64_t>(b) * p.num_heads + head0) * D;
+    finish_pair<kWarps, D, kUnit, false>(p, states, kRows, sh_last, out, len, t_first, t_last, use.left, share, seg_u,
+                                         [](float v) { return O::narrow(v); });
     __syncthreads();   // the states may be overwritten now
   }
   asm volatile("cp.async.wait_group 0;" ::: "memory");
@@ -519,7 +520,9 @@ int launch_paged_attn_mma(void* out, const void* q, const void* k_cache, const v
   p.scale_log2e = mod.softcap > 0.0f ? scale / mod.softcap : scale * 1.4426950408889634f;
   p.cap_log2e = mod.softcap * 1.4426950408889634f;
   p.slopes = mod.slopes;
-  if (dt == 1) return mod.any() ? launch_t<__half, true>(p, head_dim, sm_count, pdl, stream) : launch_t<__half, false>(p, head_dim, sm_count, pdl, stream);
+  if (dt == 1)
+    return mod.any() ? launch_t<__half, true>(p, head_dim, sm_count, pdl, stream)
+                     : launch_t<__half, false>(p, head_dim, sm_count, pdl, stream);
   return mod.any() ? launch_t<__nv_bfloat16, true>(p, head_dim, sm_count, pdl, stream)
                    : launch_t<__nv_bfloat16, false>(p, head_dim, sm_count, pdl, stream);
 }

@@ -239,9 +239,10 @@ prefill_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
   const int b = last_at_or_below(slot, p.batch, [&](int i) { return static_cast<int64_t>(__ldg(p.cu + i) / p.rows) + i; });
   if (b < 0) return;
   const int c0 = __ldg(p.cu + b), c1 = __ldg(p.cu + b + 1);
+  if (c0 < 0 || c1 <= c0 || c1 > p.tokens) return;
   const int n = c1 - c0;
   const int first_row = (slot - (c0 / p.rows + b)) * p.rows;
-  if (c0 < 0 || c1 > p.tokens || n <= 0 || first_row < 0 || first_row >= n) return;
+  if (first_row < 0 || first_row >= n) return;
   const int prefix = p.prefix ? min(n, max(0, __ldg(p.prefix + b))) : 0;
   const auto tile_at = [&](int i) {
     TileAt t;
@@ -544,8 +545,9 @@ int launch_d(const PrefillArgs& a, PrefillParams p, cudaStream_t stream) {
   p.slots = static_cast<int>(slots);
   CUtensorMap mq, mk, mv;
   int rc = make_tensor_map_2d(&mq, a.q, 2, a.tokens, static_cast<uint64_t>(a.heads) * D, a.q_stride * 2, kTile, 64, true);
-  if (rc == INFEROP_OK) rc = make_tensor_map_2d(&mk, a.k, 2, a.tokens, static_cast<uint64_t>(a.kv_heads) * D, a.k_stride * 2, C::kBlock, 64, true);
-  if (rc == INFEROP_OK) rc = make_tensor_map_2d(&mv, a.v, 2, a.tokens, static_cast<uint64_t>(a.kv_heads) * D, a.v_stride * 2, C::kBlock, 64, true);
+  const uint64_t kv_cols = static_cast<uint64_t>(a.kv_heads) * D;
+  if (rc == INFEROP_OK) rc = make_tensor_map_2d(&mk, a.k, 2, a.tokens, kv_cols, a.k_stride * 2, C::kBlock, 64, true);
+  if (rc == INFEROP_OK) rc = make_tensor_map_2d(&mv, a.v, 2, a.tokens, kv_cols, a.v_stride * 2, C::kBlock, 64, true);
   if (rc != INFEROP_OK) return rc;
   kernel<<<static_cast<unsigned>(slots * p.groups), kThreads, C::kSmemBytes, stream>>>(mq, mk, mv, p);
   return check_launch();

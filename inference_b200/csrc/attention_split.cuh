@@ -144,8 +144,8 @@ struct UnitList {
 // out: the pair's first row; t_first, t_last: first and last unit's first token; left: units of the CTA behind this pair;
 // seg_u: list index of the first unit.  kZeroIfNone: a pair without any weight gives zeros (else 0 / 0).
 template <int kWarps, int D, int kUnit, bool kZeroIfNone, typename T, typename Narrow>
-__device__ __forceinline__ void finish_pair(const AttnWork& p, float* states, int rows, int& sh_last, T* out, int len, int t_first, int t_last,
-                                            int left, long long share, long long seg_u, Narrow narrow) {
+__device__ __forceinline__ void finish_pair(const AttnWork& p, float* states, int rows, int& sh_last, T* out, int len, int t_first,
+                                            int t_last, int left, long long share, long long seg_u, Narrow narrow) {
   constexpr int kThreads = 32 * kWarps, kRec = D + 2, kPart = kAttnRows * (D + 2);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   __syncthreads();
@@ -198,7 +198,8 @@ __device__ __forceinline__ void finish_pair(const AttnWork& p, float* states, in
       float2 v[kHeads];
 #pragma unroll
       for (int e = 0; e < kHeads; ++e)
-        if (warp + e * kWarps < p.gt) v[e] = __ldcg(reinterpret_cast<const float2*>(part(i) + kAttnRows * D) + warp + e * kWarps);
+        if (warp + e * kWarps < p.gt)
+          v[e] = __ldcg(reinterpret_cast<const float2*>(part(i) + kAttnRows * D) + warp + e * kWarps);
 #pragma unroll
       for (int e = 0; e < kHeads; ++e) {
         if (warp + e * kWarps >= p.gt) break;

@@ -133,7 +133,7 @@ __device__ __forceinline__ Place place_of(const AppendParams& p, int64_t t) {
   int b;
   if (p.cu == nullptr) {
     b = static_cast<int>(t);
-    out.pos = max(-1, __ldg(p.seq_lens + b) - 1);
+    out.pos = max(0, __ldg(p.seq_lens + b)) - 1;
   } else {
     b = last_at_or_below(t, p.batch, [&](int i) { return static_cast<int64_t>(__ldg(p.cu + i)); });
     if (b < 0) return out;
@@ -316,7 +316,7 @@ __device__ __forceinline__ void block_role(const AppendParams& p, int64_t item, 
   int64_t t_first;
   if (p.cu == nullptr) {
     b = static_cast<int>(item);
-    last_pos = first_pos = __ldg(p.seq_lens + b) - 1;
+    last_pos = first_pos = max(0, __ldg(p.seq_lens + b)) - 1;
     if (first_pos < 0) return;
     j = first_pos / p.block_size;
     t_first = item;
@@ -324,9 +324,8 @@ __device__ __forceinline__ void block_role(const AppendParams& p, int64_t item, 
     b = last_at_or_below(item, p.batch, [&](int i) { return static_cast<int64_t>(__ldg(p.cu + i) / p.block_size) + 2 * i; });
     if (b < 0) return;
     const int c0 = __ldg(p.cu + b), c1 = __ldg(p.cu + b + 1);
-    const int n = c1 - c0;
-    if (n <= 0 || c0 < 0 || c1 > p.tokens) return;
-    const int len = __ldg(p.seq_lens + b);
+    if (c0 < 0 || c1 <= c0 || c1 > p.tokens) return;
+    const int n = c1 - c0, len = max(0, __ldg(p.seq_lens + b));
     last_pos = len - 1;
     first_pos = len - n;
     t_first = c0;

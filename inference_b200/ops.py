@@ -453,10 +453,6 @@ def _on_device(like: torch.Tensor, **tensors) -> None:
 
 def _append(what, q, k, v, k_cache, v_cache, scales, block_tables, seq_lens, rotary_dim, base, yarn_factor, cu_seqlens, q_out, k_out,
             stream):
-    if q_out is None and stream is None and \
-            _made(r := fast.rope_append(q, k, v, k_cache, v_cache, *(scales or (None, None)), block_tables, seq_lens, rotary_dim, base,
-                                        yarn_factor, cu_seqlens, k_out), what):
-        return r
     if q.dim() != 3 or k.dim() != 3 or k_cache.dim() != 4 or block_tables.dim() != 2 or q.dtype not in _TORCH2CODE:
         raise ValueError("q must be [tokens, heads, dim] (fp32/fp16/bf16), k and v [tokens, kv_heads, dim], the caches [blocks, "
                          "block_size, kv_heads, dim] and block_tables [batch, max_blocks]")
@@ -497,6 +493,10 @@ def rope_append_kv(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: t
     cu_seqlens int32 [batch + 1]: rows cu_seqlens[b] .. cu_seqlens[b + 1] - 1 are sequence b's last tokens; None: one
     token per sequence.  k_out: the rotated keys as well (what prefill_attn takes).  q_out may be q, k_out may be k.  Rows that
     are nobody's are left as they were in q_out and k_out."""
+    if q_out is None and stream is None and \
+            _made(r := fast.rope_append(q, k, v, k_cache, v_cache, None, None, block_tables, seq_lens, rotary_dim, base, yarn_factor,
+                                        cu_seqlens, k_out), "rope_append_kv"):
+        return r
     return _append("rope_append_kv", q, k, v, k_cache, v_cache, None, block_tables, seq_lens, rotary_dim, base, yarn_factor, cu_seqlens,
                    q_out, k_out, stream)
 
@@ -509,6 +509,10 @@ def rope_append_kv_fp8(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cach
 
     Scales are powers of two.  A token at the first row of a block begins the block anew; later ones let its scale grow where
     they need it, and the bytes before them move to the new one."""
+    if q_out is None and stream is None and \
+            _made(r := fast.rope_append(q, k, v, k_cache, v_cache, k_scales, v_scales, block_tables, seq_lens, rotary_dim, base,
+                                        yarn_factor, cu_seqlens, k_out), "rope_append_kv_fp8"):
+        return r
     return _append("rope_append_kv_fp8", q, k, v, k_cache, v_cache, (k_scales, v_scales), block_tables, seq_lens, rotary_dim, base,
                    yarn_factor, cu_seqlens, q_out, k_out, stream)
 
