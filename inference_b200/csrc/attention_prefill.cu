@@ -10,6 +10,8 @@
 //   * S = Q K^T and O += P V are tcgen05.mma with accumulators in tensor memory; P goes back into tensor memory, over the
 //     scores that it came from, and is the A operand from there.  A thread has a row of S: neither maximum nor sum
 //     needs a shuffle.
+//   * Where there are few tiles, a CTA has one, and its two warpgroups take the even and the odd blocks of keys, each with a
+//     maximum, a denominator and sums of its own; they are added at the end.  A long row's chain is half as long.
 //   * A V block and the next K block are one stage of a ring that TMA fills: one wait and one release per block for the
 //     warp that issues the MMAs, whose own time between two products is the tensor cores' idle time (535 -> 525 us below).
 //     V lies as it is (tokens outside): operand B with N contiguous.
@@ -44,6 +46,9 @@ constexpr int kTile = 128;                // query rows of a tile: the lanes of 
 // 168 per thread at launch, 208 for the first two groups and 88 for the last make the same sum
 constexpr int kThreads = 384;
 constexpr int kSoftmaxWarps = 8;
+constexpr int kSms = 148;
+constexpr int kMaxSorted = 32;            // prompts, a lane each
+constexpr int kMaxSortedCtas = 4;         // per SM
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRescaleAbove = 8.0f;     // powers of two that a maximum may lag behind
 
@@ -57,7 +62,7 @@ struct PCfg {
   static constexpr int kStageBytes = 2 * kBlockBytes;             // V of a block, then K of the next
   static constexpr int kStages = D == 64 ? 3 : 2;
   static constexpr int kBarOffset = kTiles * kQBytes + kStages * kStageBytes;
-  static constexpr int kSmemBytes = kBarOffset + 256 + 1024;      // (the base is rounded up to 1024)
+  static constexpr int kSmemBytes = kBarOffset + 256 + 1024 + kTile * 8;      // (the base is rounded up to 1024)
   // tensor memory: two score buffers (one per tile, or of alternate blocks), then the tiles' sums
   static constexpr int kSCol = 0, kOCol = 2 * kBlock;
   static_assert(kOCol + kTiles * D <= 512, "tensor memory");
@@ -76,6 +81,7 @@ struct PrefillParams {
   int groups;              // CTAs side by side over the heads
   int rows;                // query rows of a head per CTA
   int slots;               // CTAs over the tokens
+  int sorted;              // pieces by falling index
   float scale_log2e;       // what a product is multiplied by: to base 2 or, capped, to the cap's units
   float cap_log2e;
   int no_loads;            // test hook: the producer issues no load
@@ -96,6 +102,17 @@ __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+// (NaN is dropped, as by fmaxf)
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+__device__ __forceinline__ float max3_abs(float a, float b, float c) {
+  float d;
+  asm("max.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
 }
 template <typename T>
 struct Num;
@@ -140,7 +157,7 @@ __device__ __forceinline__ void change_scores(uint32_t (&s)[kChunks][32], const 
 #pragma unroll
     for (int c = 0; c < kChunks; ++c) {
 #pragma unroll
-      for (int e = 0; e < 32; ++e) top = fmaxf(top, fabsf(__uint_as_float(s[c][e])));
+      for (int e = 0; e < 32; e += 2) top = max3_abs(top, __uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1]));
     }
     if (__all_sync(0xFFFFFFFFu, top * fabsf(p.scale_log2e) <= 1.0f)) {   // (NaN is no hindrance: it stays NaN)
       const float2 cap2 = twice(p.cap_log2e);
@@ -195,13 +212,67 @@ __device__ __forceinline__ void change_scores(uint32_t (&s)[kChunks][32], const 
       }
     }
   } else {
+    float2 d = make_float2(static_cast<float>(ahead), static_cast<float>(ahead - 1));
 #pragma unroll
     for (int c = 0; c < kChunks; ++c) {
 #pragma unroll
-      for (int e = 0; e < 32; ++e)
-        s[c][e] = __float_as_uint(fmaf(-slope, fabsf(static_cast<float>(ahead - c * 32 - e)), __uint_as_float(s[c][e])));
+      for (int e = 0; e < 32; e += 2) {
+        s[c][e] = __float_as_uint(fmaf(-slope, fabsf(d.x), __uint_as_float(s[c][e])));
+        s[c][e + 1] = __float_as_uint(fmaf(-slope, fabsf(d.y), __uint_as_float(s[c][e + 1])));
+        d = __fadd2_rn(d, twice(-2.0f));
+      }
     }
   }
+}
+
+// ---- piece `index` of prompt b, which is rows [c0, c0 + n) (b < 0: none); the whole warp
+struct Piece {
+  int b, c0, n, index;
+};
+// (offsets out of order or out of range: an empty prompt)
+__device__ __forceinline__ int rows_of(const PrefillParams& p, int b, int* c0) {
+  const int from = __ldg(p.cu + b), to = __ldg(p.cu + b + 1);
+  *c0 = from;
+  return from < 0 || to <= from || to > p.tokens ? 0 : to - from;
+}
+// Prompt b owns slots from cu[b] / rows + b on: floor(n / rows) + 1 at least, and no sum over the prompts before.
+__device__ __forceinline__ Piece piece_by_slot(const PrefillParams& p, int slot) {
+  Piece at;
+  at.b = last_at_or_below(slot, p.batch, [&](int i) { return static_cast<int64_t>(__ldg(p.cu + i) / p.rows) + i; });
+  if (at.b < 0) return at;
+  at.n = rows_of(p, at.b, &at.c0);
+  at.index = slot - (at.c0 / p.rows + at.b);
+  if (at.index < 0 || static_cast<int64_t>(at.index) * p.rows >= at.n) at.b = -1;
+  return at;
+}
+// All prompts' pieces by falling index: what takes longest is begun first, whatever the order of the prompts (seven of 77 to
+// 1642 tokens, 16 heads of 64, cap and bias: 74 us, 88 in the prompts' order).  A piece of index t or
+// more exists sum max(0, pieces - t) times; t is found by bisection.
+__device__ __forceinline__ Piece piece_by_rank(const PrefillParams& p, int rank) {
+  const int lane = threadIdx.x & 31;
+  int c0 = 0;
+  const int n = lane < p.batch ? rows_of(p, lane, &c0) : 0;
+  const int mine = static_cast<int>((static_cast<uint32_t>(n) + p.rows - 1) / p.rows);
+  int lo = 0, hi = __reduce_max_sync(0xFFFFFFFFu, mine);   // pieces of an index >= lo: more than rank, >= hi: no more
+  int behind = 0;                                          // pieces of an index >= hi
+  while (hi - lo > 1) {
+    const int t = (lo + hi) / 2, f = __reduce_add_sync(0xFFFFFFFFu, max(0, mine - t));
+    if (f > rank) {
+      lo = t;
+    } else {
+      hi = t;
+      behind = f;
+    }
+  }
+  // (there may be no such piece: then rank - behind is no less than the prompts with more than lo pieces)
+  const uint32_t has = __ballot_sync(0xFFFFFFFFu, mine > lo);
+  const bool it = (has >> lane & 1u) && __popc(has & ((1u << lane) - 1u)) == rank - behind;
+  Piece at;
+  at.b = __ffs(__ballot_sync(0xFFFFFFFFu, it)) - 1;
+  at.c0 = __shfl_sync(0xFFFFFFFFu, c0, max(0, at.b));
+  at.n = __shfl_sync(0xFFFFFFFFu, n, max(0, at.b));
+  at.index = lo;
+  return at;
 }
 
 // where a CTA's tile i lies
@@ -209,7 +280,8 @@ struct TileAt {
   int head, q0, blocks;
 };
 
-template <typename T, int D, bool kMod>
+// kHalves: a CTA has one tile, and warpgroup and sums i take the blocks of keys j with j % 2 = i
+template <typename T, int D, bool kMod, bool kHalves>
 __global__ void __launch_bounds__(kThreads, 1)
 prefill_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                     const __grid_constant__ CUtensorMap map_v, const PrefillParams p) {
@@ -223,26 +295,23 @@ prefill_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
   uint64_t* edge = bars + 1;                   // [1]  TMA -> producer: a V block whose tail is set to zero
   uint64_t* s_full = bars + 2;                 // [2]  MMA -> softmax
   uint64_t* p_full = bars + 4;                 // [2]  softmax -> MMA (a warp each)
-  uint64_t* o_done = bars + 6;                 // [2]  MMA -> softmax
-  uint64_t* full = bars + 8;                   // [kStages]  TMA -> MMA
+  uint64_t* o_done = bars + 6;                 // [2]  MMA -> softmax: a product into the sums, but for the last
+  uint64_t* o_last = bars + 8;                 // [2]  ... the last
+  uint64_t* full = bars + 10;                  // [kStages]  TMA -> MMA
   uint64_t* empty = full + C::kStages;         // [kStages]  MMA -> TMA
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(empty + C::kStages);
   volatile uint32_t* abort_flag = tmem_slot + 1;
+  float2* merge_at = reinterpret_cast<float2*>(bars + 32);   // [row]: maximum and denominator of the odd blocks
 
   const int warp = __shfl_sync(0xFFFFFFFFu, static_cast<int>(threadIdx.x >> 5), 0);
   const int lane = threadIdx.x & 31;
 
-  // ---- this CTA's rows.  Sequence b owns slots from cu[b] / rows + b on (floor(n / rows) + 1 at least, and no sum over the
-  // sequences before); the last rows first: causal ones have the most keys.
+  // ---- this CTA's rows, a piece of p.rows of a prompt.  The last rows first: causal ones have the most keys.
   const int group_at = blockIdx.x % p.groups;
-  const int slot = p.slots - 1 - static_cast<int>(blockIdx.x / p.groups);
-  const int b = last_at_or_below(slot, p.batch, [&](int i) { return static_cast<int64_t>(__ldg(p.cu + i) / p.rows) + i; });
-  if (b < 0) return;
-  const int c0 = __ldg(p.cu + b), c1 = __ldg(p.cu + b + 1);
-  if (c0 < 0 || c1 <= c0 || c1 > p.tokens) return;
-  const int n = c1 - c0;
-  const int first_row = (slot - (c0 / p.rows + b)) * p.rows;
-  if (first_row < 0 || first_row >= n) return;
+  const int slot = static_cast<int>(blockIdx.x / p.groups);
+  const Piece at = p.sorted ? piece_by_rank(p, slot) : piece_by_slot(p, p.slots - 1 - slot);
+  if (at.b < 0) return;
+  const int b = at.b, c0 = at.c0, n = at.n, first_row = at.index * p.rows;
   const int prefix = p.prefix ? min(n, max(0, __ldg(p.prefix + b))) : 0;
   const auto tile_at = [&](int i) {
     TileAt t;
@@ -251,7 +320,9 @@ prefill_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     t.blocks = t.q0 >= n ? 0 : (min(n, max(t.q0 + kTile, prefix)) + BN - 1) / BN;
     return t;
   };
-  const TileAt t0 = tile_at(0), t1 = NT == 2 ? tile_at(1) : TileAt{0, 0, 0};
+  static_assert(NT == 2 || !kHalves, "two warpgroups");
+  constexpr int kStep = kHalves ? 2 : 1;       // from one block of a warpgroup to its next
+  const TileAt t0 = tile_at(0), t1 = NT == 1 ? TileAt{0, 0, 0} : kHalves ? t0 : tile_at(1);
   const int blocks = max(t0.blocks, t1.blocks);
   const int kv_col = t0.head / (p.heads / p.kv_heads) * D;
 
@@ -262,6 +333,7 @@ prefill_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[i], 4);
       mbar_init(&o_done[i], 1);
+      mbar_init(&o_last[i], 1);
     }
     for (int s = 0; s < C::kStages; ++s) {
       mbar_init(&full[s], 1);
@@ -289,8 +361,9 @@ prefill_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
       bool ok = true;
       if (!p.no_loads) {
         if (lane == 0) {
-          mbar_arrive_expect_tx(q_full, NT * C::kQBytes);   // (a tile without rows is loaded too: nothing of it is stored)
-          for (int i = 0; i < NT; ++i) {
+          constexpr int tiles = kHalves ? 1 : NT;
+          mbar_arrive_expect_tx(q_full, tiles * C::kQBytes);   // (a tile without rows is loaded too: nothing of it is stored)
+          for (int i = 0; i < tiles; ++i) {
             const TileAt t = i == 0 ? t0 : t1;
             for (int x = 0; x < C::kBoxes; ++x)
               tma_load_2d(smem + i * C::kQBytes + x * (kTile * 128), &map_q, q_full, t.head * D + x * 64, c0 + t.q0);
@@ -346,8 +419,8 @@ prefill_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
       const uint32_t q_addr = smem_u32(smem), ring_addr = smem_u32(ring);
       int stage = 0;
       uint32_t phase = 0;
-      auto scores = [&](int i, int j) {       // S = Q_i K_j^T
-        const uint32_t d = tmem + C::kSCol + (NT == 2 ? i : j & 1) * BN;
+      auto scores = [&](int i, int buf) {     // S = Q_i K^T
+        const uint32_t d = tmem + C::kSCol + buf * BN;
         const uint32_t k = ring_addr + stage * C::kStageBytes + C::kBlockBytes, q = q_addr + i * C::kQBytes;
         if (elect_one()) {
 #pragma unroll
@@ -356,40 +429,42 @@ prefill_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             umma_16bit_ss(d, umma_desc_k_sw128(q + (kk / 4) * (kTile * 128) + in_box),
                           umma_desc_k_sw128(k + (kk / 4) * (BN * 128) + in_box), idesc_s, kk > 0 ? 1u : 0u);
           }
-          umma_commit(&s_full[NT == 2 ? i : j & 1]);
+          umma_commit(&s_full[buf]);
         }
         __syncwarp();
       };
-      auto sums = [&](int i, int j) {         // O_i += P V_j
-        const uint32_t a = tmem + C::kSCol + (NT == 2 ? i : j & 1) * BN;
+      auto sums = [&](int i, int buf, bool first, bool last) {   // O_i += P V
+        const uint32_t a = tmem + C::kSCol + buf * BN;
         const uint32_t v = ring_addr + stage * C::kStageBytes;
         if (elect_one()) {
 #pragma unroll
           for (int kk = 0; kk < BN / 16; ++kk)
             umma_16bit_ts(tmem + C::kOCol + i * D, a + kk * 8, umma_desc_mn_sw128(v + kk * 2048, BN * 128), idesc_o,
-                          j > 0 || kk > 0 ? 1u : 0u);
-          umma_commit(&o_done[i]);
+                          !first || kk > 0 ? 1u : 0u);
+          umma_commit(last ? &o_last[i] : &o_done[i]);
         }
         __syncwarp();
       };
       const int tile_blocks[2] = {t0.blocks, t1.blocks};
       bool ok = warp_wait(q_full, 0u, abort_flag, p.status, kSiteAMmaQ);
-      // MMAs run in the order of their issue: a score buffer is written again behind the product that reads its P.  One tile per
-      // CTA: the scores of the next block are there before P is waited for.
+      // MMAs run in the order of their issue: a score buffer is written again behind the product that reads its P (waiting for that
+      // product first: 556 us for 526).  One tile per CTA: the scores of the next block are there before P is waited for.
+      constexpr bool alternate = NT == 1 || kHalves;
       for (int j = -1; ok && j < blocks; ++j) {
         ok = warp_wait(&full[stage], phase, abort_flag, p.status, kSiteAMmaFull);
         if (!ok) break;
         tc_fence_after_sync();
-        if (NT == 1 && j + 1 < blocks) scores(0, j + 1);
+        if (alternate && j + 1 < blocks) scores(0, (j + 1) & 1);
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
-          if (j >= 0 && j < tile_blocks[i]) {
-            ok = ok && warp_wait(&p_full[NT == 2 ? i : j & 1], (NT == 2 ? j : j >> 1) & 1, abort_flag, p.status, kSiteAMmaP);
+          if (j >= 0 && j < tile_blocks[i] && (!kHalves || (j & 1) == i)) {
+            const int buf = NT == 2 ? i : j & 1;
+            ok = ok && warp_wait(&p_full[buf], (alternate ? j >> 1 : j) & 1, abort_flag, p.status, kSiteAMmaP);
             if (!ok) break;
             tc_fence_after_sync();
-            sums(i, j);
+            sums(i, buf, j < kStep, j + kStep >= tile_blocks[i]);
           }
-          if (NT == 2 && j + 1 < tile_blocks[i]) scores(i, j + 1);
+          if (!alternate && j + 1 < tile_blocks[i]) scores(i, i);
         }
         if (elect_one()) umma_commit(&empty[stage]);
         __syncwarp();
@@ -413,10 +488,11 @@ prefill_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
       const float slope = kMod && p.slopes ? __ldg(p.slopes + t.head) * kLog2e : 0.0f;
       float m = -INFINITY, l = 0.0f;                         // m: what the row's exponentials are relative to, base 2
       bool ok = true;
-      for (int j = 0; j < t.blocks; ++j) {
+      int done = 0;                                          // blocks so far
+      for (int j = kHalves ? i : 0; j < t.blocks; j += kStep, ++done) {
         const int buf = NT == 2 ? i : j & 1;
         const uint32_t s_at = tmem + lanes + C::kSCol + buf * BN;
-        ok = warp_wait(&s_full[buf], (NT == 2 ? j : j >> 1) & 1, abort_flag, p.status, kSiteASoftmaxS);
+        ok = warp_wait(&s_full[buf], (NT == 2 ? done : done >> 1) & 1, abort_flag, p.status, kSiteASoftmaxS);
         if (!ok) break;
         tc_fence_after_sync();
         uint32_t s[BN / 32][32];
@@ -441,7 +517,8 @@ prefill_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
 #pragma unroll
         for (int c = 0; c < BN / 32; ++c) {
 #pragma unroll
-          for (int e = 0; e < 32; ++e) mx[e & 3] = fmaxf(mx[e & 3], __uint_as_float(s[c][e]));
+          for (int e = 0; e < 32; e += 2)
+            mx[(e >> 1) & 3] = max3(mx[(e >> 1) & 3], __uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1]));
         }
         const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * f;
         // (rows behind the prompt have no say: a prompt's bits do not depend on its neighbours)
@@ -450,9 +527,11 @@ prefill_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
           const float alpha = m_new == -INFINITY ? 1.0f : ex2(m - m_new);   // (every score so far -inf: no weight, not NaN)
           l *= alpha;
           m = m_new;
-          if (j > 0) {
-            // the product before is the last one on these sums until this warp's next arrival
-            ok = warp_wait(&o_done[i], (j - 1) & 1, abort_flag, p.status, kSiteASoftmaxO);
+          if (done > 0) {
+            // The product before is the last one on these sums until this warp's next arrival.  (The phase before it is over: the
+            // scores above were asked for behind that product.  The warps of a tile may be a block apart, so the
+            // end has a barrier of its own: there a warp may be two phases ahead, where a parity says nothing.)
+            ok = warp_wait(&o_done[i], (done - 1) & 1, abort_flag, p.status, kSiteASoftmaxO);
             if (!ok) break;
             tc_fence_after_sync();
 #pragma unroll 1
@@ -491,27 +570,58 @@ prefill_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         if (lane == 0) mbar_arrive(&p_full[buf]);
       }
       // ---- the row's sums / l
-      if (t.blocks > 0 && ok) {
-        if (warp_wait(&o_done[i], (t.blocks - 1) & 1, abort_flag, p.status, kSiteASoftmaxO)) {
-          tc_fence_after_sync();
-          const float inv = 1.0f / l;
-          T* dst = static_cast<T*>(p.out) + (static_cast<int64_t>(c0) + pos) * p.out_stride + static_cast<int64_t>(t.head) * D;
+      if (done > 0) {
+        ok = ok && warp_wait(&o_last[i], 0u, abort_flag, p.status, kSiteASoftmaxO);
+        tc_fence_after_sync();
+      }
+      // The odd blocks' sums and the even ones', through the place of Q (of which every product is done: scores are asked for a
+      // block ahead of sums): [dim][row], then the maxima and the denominators.
+      float mine = 1.0f, theirs = 0.0f;                      // weights of this thread's sums and of the others'
+      float* other = reinterpret_cast<float*>(smem) + (warp & 3) * 32 + lane;
+      if (kHalves && t.blocks > 1) {
+        if (i == 1 && ok) {
 #pragma unroll 1
           for (int c = 0; c < D; c += 32) {
             uint32_t o[32];
             tmem_ld_32x32(o_at + c, o);
             tmem_ld_wait();
             pin32(o);
-            if (pos < n) {
 #pragma unroll
-              for (int e = 0; e < 32; e += 8) {
-                uint4 w;
-                w.x = Num<T>::pack(__uint_as_float(o[e]) * inv, __uint_as_float(o[e + 1]) * inv);
-                w.y = Num<T>::pack(__uint_as_float(o[e + 2]) * inv, __uint_as_float(o[e + 3]) * inv);
-                w.z = Num<T>::pack(__uint_as_float(o[e + 4]) * inv, __uint_as_float(o[e + 5]) * inv);
-                w.w = Num<T>::pack(__uint_as_float(o[e + 6]) * inv, __uint_as_float(o[e + 7]) * inv);
-                *reinterpret_cast<uint4*>(dst + c + e) = w;
-              }
+            for (int e = 0; e < 32; ++e) other[(c + e) * kTile] = __uint_as_float(o[e]);
+          }
+          merge_at[pos - t.q0] = make_float2(m, l);
+        }
+        ok = !named_bar_or(1, 256, !ok) && ok;
+        if (i == 0 && ok) {
+          const float2 ml = merge_at[pos - t.q0];
+          const float m_all = fmaxf(m, ml.x);
+          mine = m == m_all ? 1.0f : ex2(m - m_all);
+          theirs = ml.x == m_all ? 1.0f : ex2(ml.x - m_all);
+          l = l * mine + ml.y * theirs;
+        }
+      }
+      if (done > 0 && ok && !(kHalves && i == 1)) {
+        const float inv = 1.0f / l;
+        T* dst = static_cast<T*>(p.out) + (static_cast<int64_t>(c0) + pos) * p.out_stride + static_cast<int64_t>(t.head) * D;
+#pragma unroll 1
+        for (int c = 0; c < D; c += 32) {
+          uint32_t o[32];
+          tmem_ld_32x32(o_at + c, o);
+          tmem_ld_wait();
+          pin32(o);
+          if (kHalves && t.blocks > 1) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(fmaf(__uint_as_float(o[e]), mine, other[(c + e) * kTile] * theirs));
+          }
+          if (pos < n) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 8) {
+              uint4 w;
+              w.x = Num<T>::pack(__uint_as_float(o[e]) * inv, __uint_as_float(o[e + 1]) * inv);
+              w.y = Num<T>::pack(__uint_as_float(o[e + 2]) * inv, __uint_as_float(o[e + 3]) * inv);
+              w.z = Num<T>::pack(__uint_as_float(o[e + 4]) * inv, __uint_as_float(o[e + 5]) * inv);
+              w.w = Num<T>::pack(__uint_as_float(o[e + 6]) * inv, __uint_as_float(o[e + 7]) * inv);
+              *reinterpret_cast<uint4*>(dst + c + e) = w;
             }
           }
         }
@@ -525,10 +635,10 @@ prefill_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
   if (warp == kSoftmaxWarps) tmem_dealloc(tmem, 512);
 }
 
-template <typename T, int D, bool kMod>
-int launch_d(const PrefillArgs& a, PrefillParams p, cudaStream_t stream) {
+template <typename T, int D, bool kMod, bool kHalves>
+int launch_h(const PrefillArgs& a, PrefillParams p, cudaStream_t stream) {
   using C = PCfg<D>;
-  const auto kernel = prefill_attn_kernel<T, D, kMod>;
+  const auto kernel = prefill_attn_kernel<T, D, kMod, kHalves>;
   static bool attr_done[64] = {};
   int dev = 0;
   cudaGetDevice(&dev);
@@ -537,12 +647,15 @@ int launch_d(const PrefillArgs& a, PrefillParams p, cudaStream_t stream) {
     if (e != cudaSuccess) return note_cuda_error(e);
     attr_done[dev] = true;
   }
-  p.by_heads = C::kTiles == 2 && a.heads / a.kv_heads % 2 == 0 ? 1 : 0;
+  p.by_heads = C::kTiles == 2 && !kHalves && a.heads / a.kv_heads % 2 == 0 ? 1 : 0;
   p.groups = p.by_heads ? a.heads / 2 : a.heads;
-  p.rows = p.by_heads ? kTile : C::kTiles * kTile;
+  p.rows = p.by_heads || kHalves ? kTile : C::kTiles * kTile;
   const int64_t slots = a.tokens / p.rows + a.batch;
   if (slots * p.groups > 0x7FFFFFFF) return INFEROP_ERR_LIMIT;
   p.slots = static_cast<int>(slots);
+  // In the prompts' order where all CTAs run at once, and from some four per SM on, which are balanced by themselves.  Times
+  // sorted / in order, ragged batches of 7 to 30: 0.85 to 1.01 between 1 and 4.3 CTAs per SM, 0.97 to 1.05 above.
+  p.sorted = a.batch > 1 && a.batch <= kMaxSorted && slots * p.groups > kSms && slots * p.groups <= kMaxSortedCtas * kSms ? 1 : 0;
   CUtensorMap mq, mk, mv;
   int rc = make_tensor_map_2d(&mq, a.q, 2, a.tokens, static_cast<uint64_t>(a.heads) * D, a.q_stride * 2, kTile, 64, true);
   const uint64_t kv_cols = static_cast<uint64_t>(a.kv_heads) * D;
@@ -551,6 +664,17 @@ int launch_d(const PrefillArgs& a, PrefillParams p, cudaStream_t stream) {
   if (rc != INFEROP_OK) return rc;
   kernel<<<static_cast<unsigned>(slots * p.groups), kThreads, C::kSmemBytes, stream>>>(mq, mk, mv, p);
   return check_launch();
+}
+
+template <typename T, int D, bool kMod>
+int launch_d(const PrefillArgs& a, const PrefillParams& p, cudaStream_t stream) {
+  if constexpr (PCfg<D>::kTiles == 2) {
+    // A tile per CTA as long as all of them run at once (two and one, heads of 128: 4096 tokens and 3 heads 60 and 39 us, 1000 and
+    // 8 19 and 15.5, 512 and 32 15 and 12.4; with up to two CTAs per SM 2000 and 16 36 and 29, but 8 x 400 and 8 14 and 19).
+    const int64_t pieces = (a.tokens + static_cast<int64_t>(a.batch) * (kTile - 1)) / kTile;   // at most
+    if (pieces * a.heads <= kSms) return launch_h<T, D, kMod, true>(a, p, stream);
+  }
+  return launch_h<T, D, kMod, false>(a, p, stream);
 }
 
 template <typename T, bool kMod>

@@ -146,3 +146,40 @@ def test_streams_graphs_and_views(ops):
         assert torch.equal(outs[0], want) and torch.equal(outs[1], want)
         for o in outs:
             o.zero_()
+
+
+@pytest.mark.parametrize("lens", [[77, 400, 130, 600, 1, 0, 333], [0, 129, 0], [(i * 37) % 150 for i in range(32)],
+                                  [(i * 37) % 90 for i in range(45)], [700, 700]], ids=["ragged", "one", "32", "45", "even"])
+@pytest.mark.parametrize("heads,kv,dim,mod", [(32, 8, 64, True), (27, 9, 128, False), (40, 20, 128, True), (26, 13, 256, False)])
+def test_more_tiles_than_sms_in_any_order(ops, heads, kv, dim, mod, lens):
+    """One to a dozen CTAs per SM, pairs of heads and of row tiles, batches of more prompts than a warp has lanes."""
+    q, k, v, cu = inputs(lens, heads, kv, dim, torch.float16, seed=heads, lead=5, tail=1)
+    slopes = torch.exp2(-8.0 * torch.arange(1, heads + 1, device="cuda") / heads) if mod else None
+    pre = torch.tensor([i % 4 * 60 for i in range(len(lens))], dtype=torch.int32, device="cuda") if mod else None
+    out = torch.full(q.shape, 7.0, dtype=torch.float16, device="cuda")
+    got = ops.prefill_attn(q, k, v, torch.tensor(cu, dtype=torch.int32, device="cuda"), dim ** -0.5, softcap=15.0 if mod else 0.0,
+                           alibi_slopes=slopes, prefix_lens=pre, out=out)
+    check(got, q, k, v, cu, dim ** -0.5, 15.0 if mod else 0.0, slopes, pre)
+    assert bool((got[:5] == 7).all()) and bool((got[cu[-1]:] == 7).all())
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_few_tiles_whose_blocks_of_keys_two_warpgroups_share(ops, dim):
+    """Growing and falling keys: the maximum lies in an even or an odd block, or moves; one to twelve blocks."""
+    for n, factor in ((1500, lambda t: t * 8), (1500, lambda t: (1 - t) * 8), (1281, lambda t: 1 + 7 * (t > 0.9)),
+                      (129, lambda t: 1 + 0 * t), (256, lambda t: 1 + 7 * (t < 0.5))):
+        q, k, v, cu = inputs([n], 4, 1, dim, torch.bfloat16, seed=n)
+        k = (k.float() * factor(torch.linspace(0, 1, n, device="cuda"))[:, None, None]).bfloat16()
+        got = ops.prefill_attn(q, k, v, torch.tensor(cu, dtype=torch.int32, device="cuda"), dim ** -0.5)
+        # scores up to some 400 here: probabilities to 400 x 2^-21
+        check(got, q, k, v, cu, dim ** -0.5, vmax=32.0)
+
+
+def test_warps_of_a_tile_that_are_a_block_apart(ops):
+    """Head size 256, whose warps may be a block ahead of one another: rows of one warp whose maximum grows often, the others' not."""
+    q, k, v, cu = inputs([2000], 32, 16, 256, torch.float16, seed=32, lead=5, tail=1)
+    cu_t = torch.tensor(cu, dtype=torch.int32, device="cuda")
+    q = q.clone()
+    q[5::3] *= 4
+    for _ in range(3):
+        check(ops.prefill_attn(q, k, v, cu_t, 0.0625), q, k, v, cu, 0.0625, vmax=32.0)
