@@ -187,7 +187,7 @@ paged_attn_fp8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
 
   long long share, u0;
   Cursor use;
-  if (!Units::begin(p, kBalance, use, share, u0)) return;
+  if (!Units::template begin<true>(p, kBalance, use, share, u0)) return;
   const int my_units = use.left;
   const int gpk = (p.num_heads / p.num_kv_heads) / p.gt;   // head groups per KV head
 

@@ -201,7 +201,7 @@ paged_attn_mma_kernel(const MmaAttnParams p) {
   // third slower, sqrt(10 U) between 30 % faster and 25 % slower.  With a dozen pairs and more the even share is the larger.
   long long share, u0;
   Cursor use;
-  if (!Units::begin(p, 0.2f, use, share, u0)) return;
+  if (!Units::template begin<false>(p, 0.2f, use, share, u0)) return;
 
   const int my_units = use.left;
 

@@ -132,6 +132,14 @@ def test_capped_scores_and_distance_bias(ops, kind, cap, bias, form):
         ops.set_option("attn_path", 0)
 
 
+@pytest.mark.parametrize("heads,kv,dim,lens", [(16, 8, 128, [900, 0, 1000, 1, 128, 129, 700] * 2), (8, 8, 64, [300] * 50 + [0, 777]),
+                                               (4, 2, 256, [64 * i for i in range(1, 41)])], ids=["few", "many", "large"])
+def test_shares_that_end_with_the_sequences(ops, heads, kv, dim, lens):
+    """More units of tokens than CTAs, fewer (sequence, head) pairs than CTAs: up to three units each."""
+    c = cache_case(heads, kv, dim, 16, lens, torch.bfloat16, seed=len(lens))
+    close(call(ops, c, dim ** -0.5), want_of(c, dim ** -0.5), torch.bfloat16)
+
+
 def test_without_cap_and_bias_it_is_the_plain_call(ops):
     for lens in ([40, 300], [9000, 16000, 1]):
         c = cache_case(32, 8, 128, 16, lens, torch.bfloat16, fp8=False)
