@@ -64,8 +64,11 @@ struct PCfg {
   static constexpr int kBarOffset = kTiles * kQBytes + kStages * kStageBytes;
   static constexpr int kSmemBytes = kBarOffset + 256 + 1024 + kTile * 8;      // (the base is rounded up to 1024)
   // tensor memory: two score buffers (one per tile, or of alternate blocks), then the tiles' sums
-  static constexpr int kSCol = 0, kOCol = 2 * kBlock;
-  static_assert(kOCol + kTiles * D <= 512, "tensor memory");
+  // and, where there is room, P in a place of its own: then a block's scores are asked for as soon as the last ones are read, not
+  // behind the product that reads P (head size 64: 211 -> 204 us; at 128 there is room with blocks of 80 keys: 612 us for 527)
+  static constexpr int kSCol = 0, kOCol = 2 * kBlock, kPCol = kOCol + kTiles * D;
+  static constexpr bool kOwnP = kTiles == 2 && kPCol + kTiles * kBlock / 2 <= 512;
+  static_assert(kPCol <= 512, "tensor memory");
   static_assert(kSmemBytes <= 232448, "shared memory");
 };
 
@@ -94,6 +97,7 @@ enum : uint32_t {
   kSiteAMmaQ = 0x241,
   kSiteAMmaFull = 0x242,
   kSiteAMmaP = 0x243,
+  kSiteAMmaS = 0x244,
   kSiteASoftmaxS = 0x341,
   kSiteASoftmaxO = 0x342,
 };
@@ -246,7 +250,7 @@ __device__ __forceinline__ Piece piece_by_slot(const PrefillParams& p, int slot)
   return at;
 }
 // All prompts' pieces by falling index: what takes longest is begun first, whatever the order of the prompts (seven of 77 to
-// 1642 tokens, 16 heads of 64, cap and bias: 74 us, 88 in the prompts' order).  A piece of index t or
+// 1642 tokens, 16 heads of 64, cap and bias: 74 us, 88 in the prompts' order, without the turns below).  A piece of index t or
 // more exists sum max(0, pieces - t) times; t is found by bisection.
 __device__ __forceinline__ Piece piece_by_rank(const PrefillParams& p, int rank) {
   const int lane = threadIdx.x & 31;
@@ -297,7 +301,9 @@ prefill_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
   uint64_t* p_full = bars + 4;                 // [2]  softmax -> MMA (a warp each)
   uint64_t* o_done = bars + 6;                 // [2]  MMA -> softmax: a product into the sums, but for the last
   uint64_t* o_last = bars + 8;                 // [2]  ... the last
-  uint64_t* full = bars + 10;                  // [kStages]  TMA -> MMA
+  uint64_t* s_free = bars + 10;                // [2]  softmax -> MMA (a warp each; P in a place of its own): the scores have been read
+  uint64_t* turn = bars + 12;                  // [2]  softmax -> the other tile's: its exponentials are done
+  uint64_t* full = bars + 14;                  // [kStages]  TMA -> MMA
   uint64_t* empty = full + C::kStages;         // [kStages]  MMA -> TMA
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(empty + C::kStages);
   volatile uint32_t* abort_flag = tmem_slot + 1;
@@ -321,6 +327,7 @@ prefill_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     return t;
   };
   static_assert(NT == 2 || !kHalves, "two warpgroups");
+  constexpr bool kEarly = C::kOwnP && !kHalves;   // a block's scores are asked for before the P of the block before is there
   constexpr int kStep = kHalves ? 2 : 1;       // from one block of a warpgroup to its next
   const TileAt t0 = tile_at(0), t1 = NT == 1 ? TileAt{0, 0, 0} : kHalves ? t0 : tile_at(1);
   const int blocks = max(t0.blocks, t1.blocks);
@@ -332,6 +339,8 @@ prefill_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[i], 4);
+      mbar_init(&s_free[i], 4);
+      mbar_init(&turn[i], 4);
       mbar_init(&o_done[i], 1);
       mbar_init(&o_last[i], 1);
     }
@@ -434,7 +443,7 @@ prefill_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         __syncwarp();
       };
       auto sums = [&](int i, int buf, bool first, bool last) {   // O_i += P V
-        const uint32_t a = tmem + C::kSCol + buf * BN;
+        const uint32_t a = tmem + (kEarly ? C::kPCol + buf * (BN / 2) : C::kSCol + buf * BN);
         const uint32_t v = ring_addr + stage * C::kStageBytes;
         if (elect_one()) {
 #pragma unroll
@@ -447,14 +456,27 @@ prefill_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
       };
       const int tile_blocks[2] = {t0.blocks, t1.blocks};
       bool ok = warp_wait(q_full, 0u, abort_flag, p.status, kSiteAMmaQ);
-      // MMAs run in the order of their issue: a score buffer is written again behind the product that reads its P (waiting for that
-      // product first: 556 us for 526).  One tile per CTA: the scores of the next block are there before P is waited for.
+      // Where P lies over the scores, MMAs that run in the order of their issue let a score buffer be written again behind the
+      // product that reads its P (waiting for that product first: 556 us for 526).  One tile per CTA: the scores of the
+      // next block are there before P is waited for.
       constexpr bool alternate = NT == 1 || kHalves;
       for (int j = -1; ok && j < blocks; ++j) {
         ok = warp_wait(&full[stage], phase, abort_flag, p.status, kSiteAMmaFull);
         if (!ok) break;
         tc_fence_after_sync();
         if (alternate && j + 1 < blocks) scores(0, (j + 1) & 1);
+        if constexpr (kEarly) {
+#pragma unroll
+          for (int i = 0; i < NT; ++i) {
+            if (j + 1 < tile_blocks[i]) {
+              if (j >= 0) ok = ok && warp_wait(&s_free[i], j & 1, abort_flag, p.status, kSiteAMmaS);
+              if (!ok) break;
+              tc_fence_after_sync();
+              scores(i, i);
+            }
+          }
+          if (!ok) break;
+        }
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
           if (j >= 0 && j < tile_blocks[i] && (!kHalves || (j & 1) == i)) {
@@ -464,7 +486,7 @@ prefill_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             tc_fence_after_sync();
             sums(i, buf, j < kStep, j + kStep >= tile_blocks[i]);
           }
-          if (!alternate && j + 1 < tile_blocks[i]) scores(i, i);
+          if (!alternate && !kEarly && j + 1 < tile_blocks[i]) scores(i, i);
         }
         if (elect_one()) umma_commit(&empty[stage]);
         __syncwarp();
@@ -489,9 +511,16 @@ prefill_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
       float m = -INFINITY, l = 0.0f;                         // m: what the row's exponentials are relative to, base 2
       bool ok = true;
       int done = 0;                                          // blocks so far
+      // Changed scores: the tiles take turns at their exponentials, so that one changes scores on the FMA units while the other
+      // keeps the special-function units busy (without turns they drift into step: 8192 tokens, 16 heads of 64,
+      // cap and bias 429 us, 398 with turns; plain scores 204 and 214; at head size 128, whose turns the
+      // products of the other tile make, capped 730 and 743).
+      constexpr bool kTurns = kEarly && kMod;
+      const int both = min(t0.blocks, t1.blocks);            // blocks that both tiles have
       for (int j = kHalves ? i : 0; j < t.blocks; j += kStep, ++done) {
         const int buf = NT == 2 ? i : j & 1;
         const uint32_t s_at = tmem + lanes + C::kSCol + buf * BN;
+        const uint32_t p_at = kEarly ? tmem + lanes + C::kPCol + i * (BN / 2) : s_at;
         ok = warp_wait(&s_full[buf], (NT == 2 ? done : done >> 1) & 1, abort_flag, p.status, kSiteASoftmaxS);
         if (!ok) break;
         tc_fence_after_sync();
@@ -501,6 +530,11 @@ prefill_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         tmem_ld_wait();
 #pragma unroll
         for (int c = 0; c < BN / 32; ++c) pin32(s[c]);
+        if constexpr (kEarly) {
+          tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&s_free[i]);
+        }
         if constexpr (kMod) change_scores<BN / 32>(s, p, slope, pos - j * BN, (j + 1) * BN <= pos_warp + 1 || prefix == 0);
         if ((j + 1) * BN > lim_warp) {
 #pragma unroll
@@ -521,6 +555,11 @@ prefill_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             mx[(e >> 1) & 3] = max3(mx[(e >> 1) & 3], __uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1]));
         }
         const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * f;
+        if (kEarly && done > 0) {   // the product that reads the P before, and the last one on these sums
+          ok = warp_wait(&o_done[i], (done - 1) & 1, abort_flag, p.status, kSiteASoftmaxO);
+          if (!ok) break;
+          tc_fence_after_sync();
+        }
         // (rows behind the prompt have no say: a prompt's bits do not depend on its neighbours)
         if (__any_sync(0xFFFFFFFFu, pos < n && (top > m + kRescaleAbove || m == -INFINITY))) {
           const float m_new = fmaxf(m, top);
@@ -531,9 +570,11 @@ prefill_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             // The product before is the last one on these sums until this warp's next arrival.  (The phase before it is over: the
             // scores above were asked for behind that product.  The warps of a tile may be a block apart, so the
             // end has a barrier of its own: there a warp may be two phases ahead, where a parity says nothing.)
-            ok = warp_wait(&o_done[i], (done - 1) & 1, abort_flag, p.status, kSiteASoftmaxO);
-            if (!ok) break;
-            tc_fence_after_sync();
+            if constexpr (!kEarly) {
+              ok = warp_wait(&o_done[i], (done - 1) & 1, abort_flag, p.status, kSiteASoftmaxO);
+              if (!ok) break;
+              tc_fence_after_sync();
+            }
 #pragma unroll 1
             for (int c = 0; c < D; c += 32) {
               uint32_t o[32];
@@ -545,6 +586,10 @@ prefill_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
               tmem_st_32x32(o_at + c, o);
             }
           }
+        }
+        if (kTurns && done < both && (i == 1 || done > 0)) {
+          ok = warp_wait(&turn[i], (i == 1 ? done : done - 1) & 1, abort_flag, p.status, kSiteASoftmaxS);
+          if (!ok) break;
         }
         const float ref = (m == -INFINITY ? 0.0f : m) - Num<T>::kUp;
         const float2 f2 = make_float2(f, f), ref2 = make_float2(-ref, -ref);
@@ -561,7 +606,11 @@ prefill_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             sum[e & 1] = __fadd2_rn(sum[e & 1], x);
             w[e] = Num<T>::pack(x.x, x.y);
           }
-          tmem_st_32x16(s_at + c * 16, w);
+          tmem_st_32x16(p_at + c * 16, w);
+        }
+        if (kTurns && done < both) {
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&turn[1 - i]);
         }
         l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
         tmem_st_wait();

@@ -145,7 +145,7 @@ def test_lists_that_are_not_in_order_stay_in_bounds(ops):
     assert bool((guard[:5] == 7).all()) and bool((guard[15:] == 7).all()) and ops.device_status()[0] == 0
 
 
-@pytest.mark.parametrize("what,sites", [("prefill", {0x141, 0x142, 0x241, 0x242, 0x243, 0x341, 0x342}), ("decode", {0x351})])
+@pytest.mark.parametrize("what,sites", [("prefill", {0x141, 0x142, 0x241, 0x242, 0x243, 0x244, 0x341, 0x342}), ("decode", {0x351})])
 def test_waits_run_out_cleanly_and_the_next_call_is_right(ops, what, sites):
     """No load is issued (a test hook), so nothing can arrive: every role gives up after a millisecond, and says where."""
     from inference_b200 import _capi
