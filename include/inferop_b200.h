@@ -286,8 +286,8 @@ INFEROP_API int inferop_paged_attn_decode_fp8(void* out, const void* q, const vo
  * any position (fp64; inferop_rope_neox multiplies in fp32), and rounded to dt once.  q goes to q_out, k to row p %
  * block_size of block block_tables[b][p / block_size] of k_cache, and to k_out; v to the same row of v_cache.
  * Not written: rows in front of cu_seqlens[0] and from cu_seqlens[batch] on and tokens without a position (p < 0); into
- * the cache, tokens beyond the table or whose entry is outside [0, num_blocks).  q_out may be q and k_out k.  The
- * sequences of a call must not share blocks that they write to.  head_dim in {64, 128, 256}. */
+ * the cache, tokens beyond the table or whose entry is outside [0, num_blocks).  q_out may be q and k_out k.  No
+ * block that a call writes to may be in its tables twice.  head_dim in {64, 128, 256}. */
 INFEROP_API int inferop_rope_append_kv(void* q_out, int64_t q_out_stride, void* k_out, int64_t k_out_stride, void* k_cache,
                               void* v_cache, const void* q, int64_t q_stride, const void* k, int64_t k_stride,
                               const void* v, int64_t v_stride, const int32_t* block_tables, const int32_t* seq_lens,

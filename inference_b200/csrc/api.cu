@@ -12,6 +12,7 @@
 #include <stdio.h>
 #include <string.h>
 
+#include <initializer_list>
 #include <mutex>
 
 #include "inferop/ops.h"
@@ -664,6 +665,13 @@ int inferop_rope_neox(void* qkv, const int64_t* positions, int32_t dt, int64_t t
                           static_cast<cudaStream_t>(stream));
 }
 
+// any of them off an address that its elements may have (null is not)
+static bool off(uintptr_t bytes, std::initializer_list<const void*> pointers) {
+  uintptr_t all = 0;
+  for (const void* p : pointers) all |= reinterpret_cast<uintptr_t>(p);
+  return (all & (bytes - 1)) != 0;
+}
+
 // The two appends: fp8 where the scales are given.
 static int kv_append(const KvAppendArgs& a, cudaStream_t s) {
   if (a.tokens <= 0 || a.batch <= 0 || a.heads <= 0 || a.kv_heads <= 0 || (a.dim != 64 && a.dim != 128 && a.dim != 256) ||
@@ -679,7 +687,10 @@ static int kv_append(const KvAppendArgs& a, cudaStream_t s) {
   if (a.heads > 65535 || a.kv_heads > 65535 || a.tokens > 0x3FFFFFFF || static_cast<int64_t>(a.max_blocks) * a.block_size > 0x7FFFFF00LL)
     return INFEROP_ERR_LIMIT;
   if (!a.q || !a.k || !a.v || !a.q_out || !a.k_cache || !a.v_cache || !a.block_tables || !a.seq_lens) return INFEROP_ERR_POINTER;
-  if ((reinterpret_cast<uintptr_t>(a.k_cache) | reinterpret_cast<uintptr_t>(a.v_cache)) & 15u) return INFEROP_ERR_POINTER;
+  if (off(16, {a.k_cache, a.v_cache}) || off(4, {a.block_tables, a.seq_lens, a.cu_seqlens, a.k_scales, a.v_scales}) ||
+      off(a.dt == 0 ? 4 : 2, {a.q, a.k, a.v, a.q_out, a.k_out})) {
+    return INFEROP_ERR_POINTER;
+  }
   int err;
   DeviceCtx* ctx = current_ctx(&err);
   if (!ctx) return err;
@@ -782,6 +793,7 @@ int inferop_paged_attn_decode_scored(void* out, const void* q, const void* k_cac
                                      int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, int32_t block_size,
                                      int32_t max_blocks_per_seq, float scale, float softcap, const float* alibi_slopes, void* stream) {
   if (!softcap_ok(softcap, scale)) return INFEROP_ERR_SHAPE;
+  if (off(4, {alibi_slopes})) return INFEROP_ERR_POINTER;
   return attn_decode(out, q, k_cache, v_cache, nullptr, block_tables, seq_lens, dt, batch, num_heads, num_kv_heads, head_dim, block_size,
                      max_blocks_per_seq, scale, ScoreMod{softcap, alibi_slopes}, stream);
 }
@@ -792,7 +804,8 @@ int inferop_paged_attn_decode_fp8(void* out, const void* q, const void* k_cache,
                                   int32_t max_blocks_per_seq, float scale, float softcap, const float* alibi_slopes, void* stream) {
   if (block_size % 16 != 0 || num_blocks <= 0 || !softcap_ok(softcap, scale)) return INFEROP_ERR_SHAPE;
   if (dt == 0) return INFEROP_ERR_DTYPE;
-  if (!k_scales || !v_scales) return INFEROP_ERR_POINTER;
+  if (!k_scales || !v_scales || off(4, {k_scales, v_scales, alibi_slopes, block_tables, seq_lens}) || off(2, {q, out}))
+    return INFEROP_ERR_POINTER;
   const Fp8Cache fp8 = {static_cast<const float*>(k_scales), static_cast<const float*>(v_scales), num_blocks};
   return attn_decode(out, q, k_cache, v_cache, &fp8, block_tables, seq_lens, dt, batch, num_heads, num_kv_heads, head_dim, block_size,
                      max_blocks_per_seq, scale, ScoreMod{softcap, alibi_slopes}, stream);
@@ -811,8 +824,8 @@ int inferop_prefill_attn(void* out, int64_t out_stride, const void* q, int64_t q
   if (dt != 1 && dt != 2) return INFEROP_ERR_DTYPE;
   if (tokens > 0x7FFFFF00LL || num_heads > 65535) return INFEROP_ERR_LIMIT;
   if (!out || !q || !k || !v || !cu_seqlens) return INFEROP_ERR_POINTER;
-  if (((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) |
-        reinterpret_cast<uintptr_t>(v)) & 15u) || ((out_stride | q_stride | k_stride | v_stride) & 7)) {
+  if (off(16, {out, q, k, v}) || off(4, {cu_seqlens, prefix_lens, alibi_slopes}) ||
+      ((out_stride | q_stride | k_stride | v_stride) & 7) != 0) {
     return INFEROP_ERR_POINTER;
   }
   int err;

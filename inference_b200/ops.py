@@ -492,7 +492,7 @@ def rope_append_kv(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: t
     contiguous); caches [blocks, block_size, kv_heads, dim]; seq_lens int32 [batch], the lengths with the new tokens.
     cu_seqlens int32 [batch + 1]: rows cu_seqlens[b] .. cu_seqlens[b + 1] - 1 are sequence b's last tokens; None: one
     token per sequence.  k_out: the rotated keys as well (what prefill_attn takes).  q_out may be q, k_out may be k.  Rows that
-    are nobody's are left as they were in q_out and k_out."""
+    are nobody's are left as they were in q_out and k_out.  No block that is written to may be in the tables twice."""
     if q_out is None and stream is None and \
             _made(r := fast.rope_append(q, k, v, k_cache, v_cache, None, None, block_tables, seq_lens, rotary_dim, base, yarn_factor,
                                         cu_seqlens, k_out), "rope_append_kv"):

@@ -182,3 +182,35 @@ def test_two_devices_or_one(ops):
         ops.prefill_attn(h, k, k.cpu(), torch.zeros(2, dtype=torch.int32, device="cuda"), 0.1)
     with pytest.raises(ValueError):
         ops.prefill_attn(h, k, k, torch.zeros(2, dtype=torch.int32), 0.1)
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+def test_caches_whose_offsets_pass_32_bits(ops, fp8):
+    """Blocks at the end of caches of more than 2^32 elements: append, then attention, against 64 bits."""
+    kv, dim, block = 8, 256, 16
+    blocks = 2 ** 32 // (block * kv * dim) + 8
+    if torch.cuda.mem_get_info()[0] < 5 * blocks * block * kv * dim:
+        pytest.skip("needs 22 GB")
+    kind = torch.uint8 if fp8 else torch.bfloat16
+    k_cache, v_cache = (torch.empty(blocks, block, kv, dim, dtype=kind, device="cuda") for _ in range(2))
+    scales = [torch.zeros(blocks, kv, device="cuda") for _ in range(2)] if fp8 else None
+    tables = torch.tensor([[blocks - 1, blocks - 3, 0], [blocks - 2, 1, blocks - 4]], dtype=torch.int32, device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(1)
+    q, k, v = (torch.randn(76, h, dim, generator=g, device="cuda").bfloat16() for h in (8, kv, kv))
+    lens, cu = torch.tensor([40, 36], dtype=torch.int32, device="cuda"), torch.tensor([0, 40, 76], dtype=torch.int32, device="cuda")
+    if fp8:
+        q = ops.rope_append_kv_fp8(q, k, v, k_cache, v_cache, *scales, tables, lens, dim, cu_seqlens=cu)[[39, 75]]
+        got = ops.paged_attn_decode_fp8(q, k_cache, v_cache, *scales, tables, lens, dim ** -0.5)
+    else:
+        q = ops.rope_append_kv(q, k, v, k_cache, v_cache, tables, lens, dim, cu_seqlens=cu)[[39, 75]]
+        got = ops.paged_attn_decode(q, k_cache, v_cache, tables, lens, dim ** -0.5, softcap=50.0)
+    for b, n in enumerate((40, 36)):
+        kk, vv = (history(c, scales[i] if fp8 else None, tables[b], n) for i, c in enumerate((k_cache, v_cache)))
+        near(got[b:b + 1], attention(q[b:b + 1], kk, vv, dim ** -0.5, 0.0 if fp8 else 50.0, None, None, None), None, torch.bfloat16, False)
+        first = cu[b].item()
+        if fp8:
+            step = scales[1][tables[b].long()][:, None].expand(3, block, kv).reshape(-1, kv)[:n, :, None].double()
+            bound = v[first:first + n].double().abs() / 16 + step * 2.0 ** -10    # half a step of E4M3, half a step of its subnormals
+            assert bool(((vv - v[first:first + n].double()).abs() <= bound).all())
+        else:
+            assert torch.equal(vv, v[first:first + n].double())

@@ -44,9 +44,12 @@ def test_appends(fp8):
     assert append(fp8, tokens=1 << 31) == _capi.ERR_LIMIT
     for name in ("q", "k", "v", "q_out", "k_cache", "v_cache", "tables", "lens"):
         assert append(fp8, **{name: None}) == _capi.ERR_POINTER, name
-    assert append(fp8, k_cache=24) == _capi.ERR_POINTER
+    for bad in (dict(k_cache=24), dict(v_cache=8), dict(tables=18), dict(lens=17), dict(cu=18), dict(q=17), dict(k=19), dict(v=17),
+                dict(k_out=17), dict(q_out=17), dict(q=18, dt=0)):
+        assert append(fp8, **bad) == _capi.ERR_POINTER, bad
     if fp8:
         assert append(True, block=24) == _capi.ERR_SHAPE
+        assert append(True, k_scales=18) == append(True, v_scales=17) == _capi.ERR_POINTER
         assert append(True, k_scales=None) == _capi.ERR_POINTER and append(True, v_scales=None) == _capi.ERR_POINTER
 
 
@@ -67,6 +70,7 @@ def test_scored_and_8_bit_decode():
     assert scored(heads=6) == fp8(heads=6) == _capi.ERR_SHAPE
     assert scored(dt=3) == fp8(dt=3) == fp8(dt=0) == _capi.ERR_DTYPE
     assert fp8(dim=32) == fp8(block=8) == fp8(block=0) == fp8(blocks=0) == _capi.ERR_SHAPE
+    assert fp8(scales=18) == _capi.ERR_POINTER
     assert fp8(scales=None) == fp8(cache=None) == fp8(cache=24) == _capi.ERR_POINTER
     assert fp8(block=1 << 20, blocks=1 << 11) == fp8(per=1 << 28) == _capi.ERR_LIMIT
 
@@ -83,7 +87,7 @@ def test_prompt_attention():
                 dict(vs=504), dict(os=1016)):
         assert call(**bad) == _capi.ERR_SHAPE, bad
     assert call(dt=0) == call(dt=3) == _capi.ERR_DTYPE
-    for bad in (dict(q=None), dict(out=None), dict(cu=None), dict(q=24), dict(qs=1028), dict(os=1025)):
+    for bad in (dict(q=None), dict(out=None), dict(cu=None), dict(cu=18), dict(q=24), dict(qs=1028), dict(os=1025)):
         assert call(**bad) == _capi.ERR_POINTER, bad
     assert call(tokens=1 << 31) == _capi.ERR_LIMIT
 
