@@ -718,10 +718,14 @@ int launch_h(const PrefillArgs& a, PrefillParams p, cudaStream_t stream) {
 template <typename T, int D, bool kMod>
 int launch_d(const PrefillArgs& a, const PrefillParams& p, cudaStream_t stream) {
   if constexpr (PCfg<D>::kTiles == 2) {
-    // A tile per CTA as long as all of them run at once (two and one, heads of 128: 4096 tokens and 3 heads 60 and 39 us, 1000 and
-    // 8 19 and 15.5, 512 and 32 15 and 12.4; with up to two CTAs per SM 2000 and 16 36 and 29, but 8 x 400 and 8 14 and 19).
+    // A tile per CTA where the longest chain decides, not the sum of the work: all CTAs at once, or, the longer the prompts, up to
+    // two to three per SM.  Two tiles and one, causal, heads of 128: 512 tokens and 32 heads 15 and 12.4 us, 1000 and 8
+    // 19 and 15.5, 4096 and 3 60 and 39; two CTAs per SM: 4096 and 8 64 and 43, 2000 and 16 35 and 30, 4 x 1200 and 6 25.5 and
+    // 24.8, but 1000 and 32 21.6 and 23, 8 x 400 and 8 14 and 19; more: 8192 and 6 122 and 111, 4096 and 12 66 and 68, 2000
+    // and 24 37 and 46, 8192 and 8 120 and 135.
     const int64_t pieces = (a.tokens + static_cast<int64_t>(a.batch) * (kTile - 1)) / kTile;   // at most
-    if (pieces * a.heads <= kSms) return launch_h<T, D, kMod, true>(a, p, stream);
+    const int64_t mean = a.tokens / a.batch / kTile;
+    if (pieces * a.heads * 2 <= (mean >= 64 ? 6 : mean >= 32 ? 5 : mean >= 9 ? 4 : 2) * kSms) return launch_h<T, D, kMod, true>(a, p, stream);
   }
   return launch_h<T, D, kMod, false>(a, p, stream);
 }

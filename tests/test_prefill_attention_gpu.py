@@ -164,6 +164,16 @@ def test_more_tiles_than_sms_in_any_order(ops, heads, kv, dim, mod, lens):
 
 
 @pytest.mark.parametrize("dim", [64, 128])
+def test_two_rounds_of_shared_tiles(ops, dim):
+    """Prompts long enough that one tile per CTA pays with up to two CTAs per SM, the longest first."""
+    lens = [1152, 1300, 1, 2200]
+    q, k, v, cu = inputs(lens, 7, 7, dim, torch.bfloat16, seed=dim, lead=2)
+    slopes = torch.rand(7, device="cuda")
+    got = ops.prefill_attn(q, k, v, torch.tensor(cu, dtype=torch.int32, device="cuda"), dim ** -0.5, alibi_slopes=slopes)
+    check(got, q, k, v, cu, dim ** -0.5, 0.0, slopes)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
 def test_few_tiles_whose_blocks_of_keys_two_warpgroups_share(ops, dim):
     """Growing and falling keys: the maximum lies in an even or an odd block, or moves; one to twelve blocks."""
     for n, factor in ((1500, lambda t: t * 8), (1500, lambda t: (1 - t) * 8), (1281, lambda t: 1 + 7 * (t > 0.9)),
