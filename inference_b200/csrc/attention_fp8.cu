@@ -568,8 +568,8 @@ int launch_paged_attn_fp8(DeviceCtx* ctx, void* out, const void* q, const void* 
   p.wide = head_dim <= 128 && block_size % 32 == 0 ? 1 : 0;
   const uint32_t box_rows = p.wide ? 32 : 16;
   CUtensorMap mk, mv;
-  int rc = make_tensor_map_2d_swizzled(&mk, k_cache, 1, rows, cols, cols, box_rows, box, box);
-  if (rc == INFEROP_OK) rc = make_tensor_map_2d_swizzled(&mv, v_cache, 1, rows, cols, cols, box_rows, box, box);
+  int rc = make_tensor_map_2d_scattered(&mk, k_cache, 1, rows, cols, cols, box_rows, box, box);
+  if (rc == INFEROP_OK) rc = make_tensor_map_2d_scattered(&mv, v_cache, 1, rows, cols, cols, box_rows, box, box);
   if (rc != INFEROP_OK) return rc;
   const int sms = ctx->sm_count;
   if (dt == 1)

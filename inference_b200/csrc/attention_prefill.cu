@@ -23,7 +23,7 @@
 // the sum is rounded to the same type at the end anyway; row sums are of the unrounded values, in fp32.
 //
 // Bound by the tensor cores and, between a tile's two products, by the chain of its softmax: 8192 tokens, 32 heads over 8 KV
-// heads of 128, bf16, causal: 525 us = 1046 TFLOP/s in long runs; a pair of blocks (256 rows, 128 keys) takes about 3400 cycles, of
+// heads of 128, bf16, causal: 525 us = 1046 TFLOP/s in long runs (at the power cap, 1.67 GHz; 460 us after a pause); a pair of blocks (256 rows, 128 keys) takes about 3400 cycles, of
 // which the products are 2048 and the softmax of a tile, which the other tile's products run beside, 1850.  Not faster:
 // blocks of 64 keys with two score buffers per tile (products of 64 columns run at half the rate: 640 us), a quarter of the
 // exponentials by polynomials (558), P handed over in halves (546), two threads per row (564), an MMA warp per tile (600).

@@ -297,8 +297,9 @@ int launch_gemm_decode_fused(DeviceCtx* ctx, float* workspace, int* counters, vo
 int make_tensor_map_2d(CUtensorMap* out, const void* base, int elem_bytes, uint64_t rows,
                        uint64_t cols, uint64_t pitch_bytes, uint32_t box_rows, uint32_t box_cols,
                        bool swizzle128);
-// the same with the swizzle by its width: 128, 64 or 0 (none)
-int make_tensor_map_2d_swizzled(CUtensorMap* out, const void* base, int elem_bytes, uint64_t rows, uint64_t cols,
-                                uint64_t pitch_bytes, uint32_t box_rows, uint32_t box_cols, int swizzle_bytes);
+// the same for small boxes that lie far apart (no more than 128 bytes of a row are fetched into L2), with the swizzle by its
+// width: 128, 64 or 0 (none)
+int make_tensor_map_2d_scattered(CUtensorMap* out, const void* base, int elem_bytes, uint64_t rows, uint64_t cols,
+                                 uint64_t pitch_bytes, uint32_t box_rows, uint32_t box_cols, int swizzle_bytes);
 
 }  // namespace ib200

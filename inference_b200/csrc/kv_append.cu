@@ -310,7 +310,7 @@ __device__ __forceinline__ float value_of(uint8_t byte) {
 // floor(n / block_size) + 2 blocks, and the bound needs no sum over the sequences before.
 template <typename T, int V>
 __device__ __forceinline__ void block_role(const AppendParams& p, int64_t item, float2* cs) {
-  __shared__ float amax_of[2][64];   // several chunks of tokens: maximum so far of (kind, head) of this round
+  __shared__ float amax_of[2][64];   // several chunks of tokens: maximum so far of (kind, head) of this set of heads
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int b, first_pos, last_pos, j;     // the sequence's new positions [first_pos, last_pos], the block among its own
   int64_t t_first;
@@ -391,7 +391,7 @@ __device__ __forceinline__ void block_role(const AppendParams& p, int64_t item, 
       turn<V>(t, x0, x1);
     }
   };
-  // (rounds of 64 heads, so that the maxima have a place whatever the number of heads)
+  // (64 heads at a time, so that the maxima have a place whatever the number of heads)
   for (int h0 = 0; h0 < p.kv_heads; h0 += 64) {
     const int jobs = 2 * min(64, p.kv_heads - h0);
     for (int step = 0; step < (chunks == 1 ? 1 : 2 * chunks); ++step) {

@@ -30,16 +30,8 @@ EncodeFn encode_fn() {
   return fn;
 }
 
-}  // namespace
-
-int make_tensor_map_2d(CUtensorMap* out, const void* base, int elem_bytes, uint64_t rows,
-                       uint64_t cols, uint64_t pitch_bytes, uint32_t box_rows, uint32_t box_cols,
-                       bool swizzle128) {
-  return make_tensor_map_2d_swizzled(out, base, elem_bytes, rows, cols, pitch_bytes, box_rows, box_cols, swizzle128 ? 128 : 0);
-}
-
-int make_tensor_map_2d_swizzled(CUtensorMap* out, const void* base, int elem_bytes, uint64_t rows, uint64_t cols,
-                                uint64_t pitch_bytes, uint32_t box_rows, uint32_t box_cols, int swizzle_bytes) {
+int encode(CUtensorMap* out, const void* base, int elem_bytes, uint64_t rows, uint64_t cols, uint64_t pitch_bytes, uint32_t box_rows,
+           uint32_t box_cols, int swizzle_bytes, CUtensorMapL2promotion promotion) {
   EncodeFn fn = encode_fn();
   if (!fn) return INFEROP_ERR_CUDA;
   if ((reinterpret_cast<uintptr_t>(base) & 15u) != 0 || (pitch_bytes & 15u) != 0) {
@@ -55,14 +47,29 @@ int make_tensor_map_2d_swizzled(CUtensorMap* out, const void* base, int elem_byt
   const CUresult r =
       fn(out, type, 2, const_cast<void*>(base), dims, strides, box, elem_strides,
          CU_TENSOR_MAP_INTERLEAVE_NONE,
-         swizzle_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B
-         : swizzle_bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_NONE,
-         elem_bytes == 1 && box_rows <= 32 ? CU_TENSOR_MAP_L2_PROMOTION_L2_128B : CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+         swizzle_bytes == 128  ? CU_TENSOR_MAP_SWIZZLE_128B
+         : swizzle_bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
+                               : CU_TENSOR_MAP_SWIZZLE_NONE,
+         promotion, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) {
     note_cuda_error(cudaErrorInvalidValue);
     return INFEROP_ERR_CUDA;
   }
   return INFEROP_OK;
+}
+
+}  // namespace
+
+int make_tensor_map_2d(CUtensorMap* out, const void* base, int elem_bytes, uint64_t rows,
+                       uint64_t cols, uint64_t pitch_bytes, uint32_t box_rows, uint32_t box_cols,
+                       bool swizzle128) {
+  return encode(out, base, elem_bytes, rows, cols, pitch_bytes, box_rows, box_cols, swizzle128 ? 128 : 0,
+                CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
+}
+
+int make_tensor_map_2d_scattered(CUtensorMap* out, const void* base, int elem_bytes, uint64_t rows, uint64_t cols,
+                                 uint64_t pitch_bytes, uint32_t box_rows, uint32_t box_cols, int swizzle_bytes) {
+  return encode(out, base, elem_bytes, rows, cols, pitch_bytes, box_rows, box_cols, swizzle_bytes, CU_TENSOR_MAP_L2_PROMOTION_L2_128B);
 }
 
 }  // namespace ib200

@@ -214,3 +214,24 @@ def test_caches_whose_offsets_pass_32_bits(ops, fp8):
             assert bool(((vv - v[first:first + n].double()).abs() <= bound).all())
         else:
             assert torch.equal(vv, v[first:first + n].double())
+
+
+@pytest.mark.parametrize("dim,cap", [(64, 0.0), (64, 20.0), (128, 0.0), (256, 0.0)])
+def test_prompt_waits_run_out_cleanly_with_two_tiles_per_cta(ops, dim, cap):
+    """More tiles than SMs: pairs of tiles (taking turns where scores are capped), or the form of the largest heads."""
+    from inference_b200 import _capi
+    q = torch.randn(300, 80, dim, device="cuda").half()
+    k = torch.randn(300, 40, dim, device="cuda").half()
+    cu = torch.tensor([0, 300], dtype=torch.int32, device="cuda")
+    want = ops.prefill_attn(q, k, k, cu, 0.1, softcap=cap)
+    rec = (C.c_uint32 * 4)()
+    try:
+        ops.set_option("wait_budget_us", 1000)
+        ops.set_option("debug_no_loads", 1)
+        ops.prefill_attn(q, k, k, cu, 0.1, softcap=cap)
+        rc = _capi.lib.inferop_device_status(rec, 1)
+        assert rc == _capi.ERR_DEVICE_WAIT and rec[0] in {0x241, 0x242, 0x341, 0x342}, (rc, [hex(v) for v in rec])
+    finally:
+        ops.set_option("debug_no_loads", 0)
+        ops.set_option("wait_budget_us", 0)
+    assert torch.equal(ops.prefill_attn(q, k, k, cu, 0.1, softcap=cap), want) and ops.device_status()[0] == 0
