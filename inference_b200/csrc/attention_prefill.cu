@@ -23,8 +23,9 @@
 // the sum is rounded to the same type at the end anyway; row sums are of the unrounded values, in fp32.
 //
 // Bound by the tensor cores and, between a tile's two products, by the chain of its softmax: 8192 tokens, 32 heads over 8 KV
-// heads of 128, bf16, causal: 525 us = 1046 TFLOP/s in long runs (at the power cap, 1.67 GHz; 460 us after a pause); a pair of blocks (256 rows, 128 keys) takes about 3400 cycles, of
-// which the products are 2048 and the softmax of a tile, which the other tile's products run beside, 1850.  Not faster:
+// heads of 128, bf16, causal: 525 us = 1046 TFLOP/s in long runs (at the power cap, 1.67 GHz; 460 us after a pause).  A pair of
+// blocks (256 rows, 128 keys) takes about 3400 cycles, of which the products are 2048 and the softmax of a tile, which the other
+// tile's products run beside, 1850.  Not faster:
 // blocks of 64 keys with two score buffers per tile (products of 64 columns run at half the rate: 640 us), a quarter of the
 // exponentials by polynomials (558), P handed over in halves (546), two threads per row (564), an MMA warp per tile (600).
 #include <cuda_bf16.h>
@@ -725,7 +726,8 @@ int launch_d(const PrefillArgs& a, const PrefillParams& p, cudaStream_t stream) 
     // and 24 37 and 46, 8192 and 8 120 and 135.
     const int64_t pieces = (a.tokens + static_cast<int64_t>(a.batch) * (kTile - 1)) / kTile;   // at most
     const int64_t mean = a.tokens / a.batch / kTile;
-    if (pieces * a.heads * 2 <= (mean >= 64 ? 6 : mean >= 32 ? 5 : mean >= 9 ? 4 : 2) * kSms) return launch_h<T, D, kMod, true>(a, p, stream);
+    const int half_ctas = mean >= 64 ? 6 : mean >= 32 ? 5 : mean >= 9 ? 4 : 2;                 // per SM
+    if (pieces * a.heads * 2 <= half_ctas * kSms) return launch_h<T, D, kMod, true>(a, p, stream);
   }
   return launch_h<T, D, kMod, false>(a, p, stream);
 }

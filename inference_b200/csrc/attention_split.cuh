@@ -83,7 +83,7 @@ struct UnitList {
   // about sqrt(U / balance) CTAs, where a unit's time and a part's balance.
   // kAligned: where a little larger share lets every CTA end with a pair or before, it is taken: a pair is then as many CTAs'
   // worth of units (the last one's partly void), and no CTA pays for the end of one pair and the start of another (E4M3, 32
-  // heads over 8 of 128, tokens each: 16 x 1000 23.4 -> 16.8 us, 48 x 1000 31.7 -> 26.4, 8 x 4096 26.6 -> 24.7; calls
+  // heads over 8 of 128, one cache as K and V: 16 x 1000 23.4 -> 16.8 us, 48 x 1000 31.7 -> 26.4, 8 x 4096 26.6 -> 24.7; calls
   // that are cut the same either way pay 0.2 to 0.6 us for the decision).
   template <bool kAligned>
   static __device__ __forceinline__ bool begin(const AttnWork& p, float balance, Cursor& use, long long& share, long long& u0) {

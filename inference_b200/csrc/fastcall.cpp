@@ -376,8 +376,8 @@ PyObject* paged_attn_decode_scored(PyObject*, PyObject* const* a, Py_ssize_t n) 
                                          i32(batch), i32(heads), i32(kv), i32(dim), i32(block), i32(blocks), i32(per), scale, cap, sl_ptr,
                                          stream_of(dev));
     } else {
-      rc = inferop_paged_attn_decode_scored(out.data_ptr(), q->data_ptr(), kc->data_ptr(), vc->data_ptr(), ints(bt), ints(sl), dt, i32(batch),
-                                            i32(heads), i32(kv), i32(dim), i32(block), i32(per), scale, cap, sl_ptr, stream_of(dev));
+      rc = inferop_paged_attn_decode_scored(out.data_ptr(), q->data_ptr(), kc->data_ptr(), vc->data_ptr(), ints(bt), ints(sl), dt,
+                                            i32(batch), i32(heads), i32(kv), i32(dim), i32(block), i32(per), scale, cap, sl_ptr, stream_of(dev));
     }
   }
   if (rc != INFEROP_OK) return PyLong_FromLong(rc);
@@ -421,7 +421,8 @@ PyObject* prefill_attn(PyObject*, PyObject* const* a, Py_ssize_t n) {
 
 #define FAST(f) {#f, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {FAST(quant), FAST(gemm), FAST(gemm_fused_quant), FAST(rmsnorm_quant), FAST(rope_neox),
-                         FAST(paged_attn_decode), FAST(rope_append), FAST(paged_attn_decode_scored), FAST(prefill_attn), {nullptr, nullptr, 0, nullptr}};
+                         FAST(paged_attn_decode), FAST(rope_append), FAST(paged_attn_decode_scored), FAST(prefill_attn),
+                         {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_fastcall", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -235,3 +235,37 @@ def test_prompt_waits_run_out_cleanly_with_two_tiles_per_cta(ops, dim, cap):
         ops.set_option("debug_no_loads", 0)
         ops.set_option("wait_budget_us", 0)
     assert torch.equal(ops.prefill_attn(q, k, k, cu, 0.1, softcap=cap), want) and ops.device_status()[0] == 0
+
+
+def test_native_calls_take_the_plain_forms_and_give_the_general_ones_bits(ops):
+    from inference_b200 import _capi
+    fast = _capi.fast
+    if not fast.__name__.endswith("_fastcall"):
+        pytest.skip("no native module for this torch")
+    g = torch.Generator(device="cuda").manual_seed(3)
+    q, k, v = (torch.randn(50, h, 64, generator=g, device="cuda").bfloat16() for h in (6, 2, 2))
+    tables = torch.arange(8, dtype=torch.int32, device="cuda").view(2, 4)
+    lens, cu = torch.tensor([30, 20], dtype=torch.int32, device="cuda"), torch.tensor([0, 30, 50], dtype=torch.int32, device="cuda")
+    slopes = torch.rand(6, device="cuda")
+    for fp8 in (False, True):
+        results = []
+        for form in (0, 1):
+            kind = torch.uint8 if fp8 else torch.bfloat16
+            kc, vc = (torch.zeros(8, 16, 2, 64, dtype=kind, device="cuda") for _ in range(2))
+            ks, vs = (torch.zeros(8, 2, device="cuda") for _ in range(2)) if fp8 else (None, None)
+            if form == 0:
+                turned = fast.rope_append(q, k, v, kc, vc, ks, vs, tables, lens, 64, 1e4, 1.0, cu, None)
+                one = turned[[29, 49]].contiguous()
+                got = fast.paged_attn_decode_scored(one, kc, vc, ks, vs, tables, lens, 0.1, 5.0, slopes)
+            else:
+                append = ops.rope_append_kv_fp8 if fp8 else ops.rope_append_kv
+                turned = append(q, k, v, kc, vc, *((ks, vs) if fp8 else ()), tables, lens, 64, cu_seqlens=cu, q_out=torch.empty_like(q))
+                one = turned[[29, 49]].contiguous()
+                decode = ops.paged_attn_decode_fp8 if fp8 else ops.paged_attn_decode
+                got = decode(one, kc, vc, *((ks, vs) if fp8 else ()), tables, lens, 0.1, softcap=5.0, alibi_slopes=slopes,
+                             out=torch.empty_like(one))
+            results.append((turned, kc, vc, got))
+        for a, b in zip(*results):
+            assert torch.is_tensor(a) and torch.equal(a, b)
+    assert torch.equal(fast.prefill_attn(q, k, v, cu, 0.1, 0.0, slopes, lens),
+                       ops.prefill_attn(q, k, v, cu, 0.1, alibi_slopes=slopes, prefix_lens=lens, out=torch.empty_like(q)))
