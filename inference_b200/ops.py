@@ -532,7 +532,7 @@ def paged_attn_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
 
     softcap > 0: scores are softcap * tanh(score / softcap).  alibi_slopes fp32 [heads]: then minus the head's slope times a
     token's distance from the last one."""
-    scored = alibi_slopes is not None or softcap != 0.0
+    scored = softcap != 0.0 or alibi_slopes is not None
     if out is None and stream is None:
         if scored:
             r = fast.paged_attn_decode_scored(q, k_cache, v_cache, None, None, block_tables, seq_lens, scale, softcap, alibi_slopes)
@@ -549,18 +549,22 @@ def paged_attn_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
     if block_tables.dtype != torch.int32 or seq_lens.dtype != torch.int32 or block_tables.dim() != 2 or \
             block_tables.shape[0] != q.shape[0] or seq_lens.numel() != q.shape[0]:
         raise ValueError("block_tables must be int32 [batch, max_blocks] and seq_lens int32 [batch]")
-    slopes = _slopes_ptr(alibi_slopes, q)
     batch, heads, dim = q.shape
     _, block_size, kv_heads, _ = k_cache.shape
     with _on(q):
         if out is None:
             out = torch.empty_like(q)
-        args = (out.data_ptr(), q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_tables.data_ptr(), seq_lens.data_ptr(),
-                _TORCH2CODE[q.dtype], batch, heads, kv_heads, dim, block_size, block_tables.shape[1], float(scale))
-        if scored:
-            check(lib.inferop_paged_attn_decode_scored(*args, float(softcap), slopes, _stream_ptr(q, stream)), "paged_attn_decode")
+        if not scored:
+            check(lib.inferop_paged_attn_decode(out.data_ptr(), q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+                                                block_tables.data_ptr(), seq_lens.data_ptr(), _TORCH2CODE[q.dtype], batch, heads,
+                                                kv_heads, dim, block_size, block_tables.shape[1], float(scale),
+                                                _stream_ptr(q, stream)), "paged_attn_decode")
         else:
-            check(lib.inferop_paged_attn_decode(*args, _stream_ptr(q, stream)), "paged_attn_decode")
+            slopes = _slopes_ptr(alibi_slopes, q)
+            check(lib.inferop_paged_attn_decode_scored(out.data_ptr(), q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+                                                       block_tables.data_ptr(), seq_lens.data_ptr(), _TORCH2CODE[q.dtype], batch, heads,
+                                                       kv_heads, dim, block_size, block_tables.shape[1], float(scale), float(softcap),
+                                                       slopes, _stream_ptr(q, stream)), "paged_attn_decode")
     return out
 
 
