@@ -339,7 +339,8 @@ paged_attn_fp8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
       if (tw < len) {
         asm volatile("cp.async.wait_group %0;" ::"n"(C::kStages - 1) : "memory");
         if (!dead) dead = !mbar_wait(&bars[slot], (phases >> slot) & 1u, &sh_abort, p.status, kSiteFp8Tiles);
-        dead = __any_sync(0xFFFFFFFFu, dead);   // (and the other lanes' copies are there too)
+        dead = __any_sync(0xFFFFFFFFu, dead);
+        __syncwarp();                           // the scales are lane 0's and 1's copies: a vote orders no memory
         phases ^= 1u << slot;
         if (!dead) {
           const uint32_t at = ring_at + slot * C::kStageBytes;

@@ -246,3 +246,18 @@ def test_graphs_and_streams_share_no_scratch(ops):
         for o in outs:
             o.zero_()
         torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("heads,kv,dim,block", [(32, 8, 128, 16), (8, 8, 64, 16), (4, 2, 256, 16), (8, 2, 128, 32)])
+def test_every_step_has_its_blocks_scales(ops, dtype, heads, kv, dim, block):
+    """Scales that differ from block to block and are no powers of two, over many steps of every warp, again and again."""
+    c = cache_case(heads, kv, dim, block, [4101, 700, 33], dtype, seed=dim + block)
+    g = torch.Generator().manual_seed(1)
+    for n in ("k_scales", "v_scales"):
+        c[n] = c[n] * (0.4 + 1.6 * torch.rand(c[n].shape, generator=g))
+    got = call(ops, c, dim ** -0.5)
+    # values up to some 40
+    close(got, want_of(c, dim ** -0.5), dtype, atol=2e-3)
+    for _ in range(20):
+        assert torch.equal(call(ops, c, dim ** -0.5), got)
