@@ -7,9 +7,12 @@
 // One pass over the keys with a running maximum and sum per query row.
 //   * A CTA has two tiles of 128 query rows (two heads of one KV head where the group is even, else 256 rows of a head; one
 //     tile at head size 256), so that the tensor cores work on one while the other's scores are exponentiated.
-//   * S = Q K^T and O += P V are tcgen05.mma with accumulators in tensor memory; P goes back into tensor memory, over the
-//     scores that it came from, and is the A operand from there.  A thread has a row of S: neither maximum nor sum
-//     needs a shuffle.
+//   * S = Q K^T and O += P V are tcgen05.mma with accumulators in tensor memory; P goes back into tensor memory and is the A
+//     operand from there.  A thread has a row of S: neither maximum nor sum needs a shuffle.
+//   * P lies beside the scores, in a place of its own: MMAs are promised to run in the order of their issue only where accumulator
+//     and shape are the same, so scores must not be written over the P that an earlier product may still read.  At head size 128
+//     tensor memory has room for that with one score buffer, which the tiles use in turn: a tile's scores are in registers
+//     soon after they are there.
 //   * Where there are few tiles, a CTA has one, and its two warpgroups take the even and the odd blocks of keys, each with a
 //     maximum, a denominator and sums of its own; they are added at the end.  A long row's chain is half as long.
 //   * A V block and the next K block are one stage of a ring that TMA fills: one wait and one release per block for the
@@ -64,12 +67,10 @@ struct PCfg {
   static constexpr int kStages = D == 64 ? 3 : 2;
   static constexpr int kBarOffset = kTiles * kQBytes + kStages * kStageBytes;
   static constexpr int kSmemBytes = kBarOffset + 256 + 1024 + kTile * 8;      // (the base is rounded up to 1024)
-  // tensor memory: two score buffers (one per tile, or of alternate blocks), then the tiles' sums
-  // and, where there is room, P in a place of its own: then a block's scores are asked for as soon as the last ones are read, not
-  // behind the product that reads P (head size 64: 211 -> 204 us; at 128 there is room with blocks of 80 keys: 612 us for 527)
-  static constexpr int kSCol = 0, kOCol = 2 * kBlock, kPCol = kOCol + kTiles * D;
-  static constexpr bool kOwnP = kTiles == 2 && kPCol + kTiles * kBlock / 2 <= 512;
-  static_assert(kPCol <= 512, "tensor memory");
+  // tensor memory: score buffers (one per tile, or of alternate blocks; head size 128: one for all), two places for P, the sums
+  static constexpr int kScoreBufs = D == 128 ? 1 : 2;
+  static constexpr int kSCol = 0, kPCol = kScoreBufs * kBlock, kOCol = kPCol + 2 * (kBlock / 2);
+  static_assert(kOCol + kTiles * D <= 512, "tensor memory");
   static_assert(kSmemBytes <= 232448, "shared memory");
 };
 
@@ -302,7 +303,7 @@ prefill_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
   uint64_t* p_full = bars + 4;                 // [2]  softmax -> MMA (a warp each)
   uint64_t* o_done = bars + 6;                 // [2]  MMA -> softmax: a product into the sums, but for the last
   uint64_t* o_last = bars + 8;                 // [2]  ... the last
-  uint64_t* s_free = bars + 10;                // [2]  softmax -> MMA (a warp each; P in a place of its own): the scores have been read
+  uint64_t* s_free = bars + 10;                // [2]  softmax -> MMA (a warp each; pairs, or one buffer): the scores have been read
   uint64_t* turn = bars + 12;                  // [2]  softmax -> the other tile's: its exponentials are done
   uint64_t* full = bars + 14;                  // [kStages]  TMA -> MMA
   uint64_t* empty = full + C::kStages;         // [kStages]  MMA -> TMA
@@ -328,7 +329,8 @@ prefill_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     return t;
   };
   static_assert(NT == 2 || !kHalves, "two warpgroups");
-  constexpr bool kEarly = C::kOwnP && !kHalves;   // a block's scores are asked for before the P of the block before is there
+  constexpr bool kPairs = NT == 2 && !kHalves;    // two tiles
+  constexpr bool kOneBuf = C::kScoreBufs == 1;    // both warpgroups' scores come into one buffer
   constexpr int kStep = kHalves ? 2 : 1;       // from one block of a warpgroup to its next
   const TileAt t0 = tile_at(0), t1 = NT == 1 ? TileAt{0, 0, 0} : kHalves ? t0 : tile_at(1);
   const int blocks = max(t0.blocks, t1.blocks);
@@ -430,7 +432,7 @@ prefill_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
       int stage = 0;
       uint32_t phase = 0;
       auto scores = [&](int i, int buf) {     // S = Q_i K^T
-        const uint32_t d = tmem + C::kSCol + buf * BN;
+        const uint32_t d = tmem + C::kSCol + (kOneBuf ? 0 : buf * BN);
         const uint32_t k = ring_addr + stage * C::kStageBytes + C::kBlockBytes, q = q_addr + i * C::kQBytes;
         if (elect_one()) {
 #pragma unroll
@@ -444,7 +446,7 @@ prefill_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         __syncwarp();
       };
       auto sums = [&](int i, int buf, bool first, bool last) {   // O_i += P V
-        const uint32_t a = tmem + (kEarly ? C::kPCol + buf * (BN / 2) : C::kSCol + buf * BN);
+        const uint32_t a = tmem + C::kPCol + buf * (BN / 2);
         const uint32_t v = ring_addr + stage * C::kStageBytes;
         if (elect_one()) {
 #pragma unroll
@@ -457,37 +459,43 @@ prefill_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
       };
       const int tile_blocks[2] = {t0.blocks, t1.blocks};
       bool ok = warp_wait(q_full, 0u, abort_flag, p.status, kSiteAMmaQ);
-      // Where P lies over the scores, MMAs that run in the order of their issue let a score buffer be written again behind the
-      // product that reads its P (waiting for that product first: 556 us for 526).  One tile per CTA: the scores of the
-      // next block are there before P is waited for.
-      constexpr bool alternate = NT == 1 || kHalves;
+      // What a product overwrites has been read: scores by s_free or, where they alternate between two buffers, by the P of the
+      // block before last.  One tile per CTA: the scores of the next block are there before P is waited for.
       for (int j = -1; ok && j < blocks; ++j) {
         ok = warp_wait(&full[stage], phase, abort_flag, p.status, kSiteAMmaFull);
         if (!ok) break;
         tc_fence_after_sync();
-        if (alternate && j + 1 < blocks) scores(0, (j + 1) & 1);
-        if constexpr (kEarly) {
-#pragma unroll
-          for (int i = 0; i < NT; ++i) {
-            if (j + 1 < tile_blocks[i]) {
-              if (j >= 0) ok = ok && warp_wait(&s_free[i], j & 1, abort_flag, p.status, kSiteAMmaS);
-              if (!ok) break;
-              tc_fence_after_sync();
-              scores(i, i);
-            }
+        const auto next_scores = [&](int i) {               // of tile i; read: the scores before in the same buffer
+          if (j + 1 >= tile_blocks[i]) return;
+          int by = i, block = j;
+          if (kOneBuf && i == 0 && j < tile_blocks[1]) by = 1;
+          if (kOneBuf && i == 1 && j + 1 < tile_blocks[0]) by = 0, block = j + 1;
+          if (block >= 0) ok = ok && warp_wait(&s_free[by], block & 1, abort_flag, p.status, kSiteAMmaS);
+          if (!ok) return;
+          tc_fence_after_sync();
+          scores(i, i);
+        };
+        if constexpr (!kPairs) {
+          if (j + 1 < blocks) {
+            if (kOneBuf && j >= 0) ok = warp_wait(&s_free[j & 1], (j >> 1) & 1, abort_flag, p.status, kSiteAMmaS);
+            if (!ok) break;
+            tc_fence_after_sync();
+            scores(0, (j + 1) & 1);
           }
-          if (!ok) break;
+        } else if (!kOneBuf) {
+#pragma unroll
+          for (int i = 0; i < NT; ++i) next_scores(i);
         }
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
+          if (kPairs && kOneBuf) next_scores(i);
           if (j >= 0 && j < tile_blocks[i] && (!kHalves || (j & 1) == i)) {
             const int buf = NT == 2 ? i : j & 1;
-            ok = ok && warp_wait(&p_full[buf], (alternate ? j >> 1 : j) & 1, abort_flag, p.status, kSiteAMmaP);
+            ok = ok && warp_wait(&p_full[buf], (kPairs ? j : j >> 1) & 1, abort_flag, p.status, kSiteAMmaP);
             if (!ok) break;
             tc_fence_after_sync();
             sums(i, buf, j < kStep, j + kStep >= tile_blocks[i]);
           }
-          if (!alternate && !kEarly && j + 1 < tile_blocks[i]) scores(i, i);
         }
         if (elect_one()) umma_commit(&empty[stage]);
         __syncwarp();
@@ -516,12 +524,12 @@ prefill_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
       // keeps the special-function units busy (without turns they drift into step: 8192 tokens, 16 heads of 64,
       // cap and bias 429 us, 398 with turns; plain scores 204 and 214; at head size 128, whose turns the
       // products of the other tile make, capped 730 and 743).
-      constexpr bool kTurns = kEarly && kMod;
+      constexpr bool kTurns = D == 64 && kPairs && kMod;
       const int both = min(t0.blocks, t1.blocks);            // blocks that both tiles have
       for (int j = kHalves ? i : 0; j < t.blocks; j += kStep, ++done) {
         const int buf = NT == 2 ? i : j & 1;
-        const uint32_t s_at = tmem + lanes + C::kSCol + buf * BN;
-        const uint32_t p_at = kEarly ? tmem + lanes + C::kPCol + i * (BN / 2) : s_at;
+        const uint32_t s_at = tmem + lanes + C::kSCol + (kOneBuf ? 0 : buf * BN);
+        const uint32_t p_at = tmem + lanes + C::kPCol + buf * (BN / 2);
         ok = warp_wait(&s_full[buf], (NT == 2 ? done : done >> 1) & 1, abort_flag, p.status, kSiteASoftmaxS);
         if (!ok) break;
         tc_fence_after_sync();
@@ -531,7 +539,7 @@ prefill_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         tmem_ld_wait();
 #pragma unroll
         for (int c = 0; c < BN / 32; ++c) pin32(s[c]);
-        if constexpr (kEarly) {
+        if constexpr (kPairs || kOneBuf) {
           tc_fence_before_sync();
           __syncwarp();
           if (lane == 0) mbar_arrive(&s_free[i]);
@@ -556,7 +564,9 @@ prefill_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             mx[(e >> 1) & 3] = max3(mx[(e >> 1) & 3], __uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1]));
         }
         const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * f;
-        if (kEarly && done > 0) {   // the product that reads the P before, and the last one on these sums
+        // The product that reads the P before in the same place has to be over.  One tile per CTA: it is that of the block before
+        // last, issued before the scores above were, whose arrival says that everything before them is done.
+        if (kPairs && done > 0) {   // (and it is the last one on these sums)
           ok = warp_wait(&o_done[i], (done - 1) & 1, abort_flag, p.status, kSiteASoftmaxO);
           if (!ok) break;
           tc_fence_after_sync();
@@ -568,10 +578,10 @@ prefill_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
           l *= alpha;
           m = m_new;
           if (done > 0) {
-            // The product before is the last one on these sums until this warp's next arrival.  (The phase before it is over: the
-            // scores above were asked for behind that product.  The warps of a tile may be a block apart, so the
+            // The product before is the last one on these sums until this warp's next arrival.  (The phase before it is over: its
+            // product was issued before the scores above were.  The warps of a tile may be a block apart, so the
             // end has a barrier of its own: there a warp may be two phases ahead, where a parity says nothing.)
-            if constexpr (!kEarly) {
+            if constexpr (!kPairs) {
               ok = warp_wait(&o_done[i], (done - 1) & 1, abort_flag, p.status, kSiteASoftmaxO);
               if (!ok) break;
               tc_fence_after_sync();

@@ -193,3 +193,15 @@ def test_warps_of_a_tile_that_are_a_block_apart(ops):
     q[5::3] *= 4
     for _ in range(3):
         check(ops.prefill_attn(q, k, v, cu_t, 0.0625), q, k, v, cu, 0.0625, vmax=32.0)
+
+
+@pytest.mark.parametrize("heads,kv,dim", [(32, 8, 128), (27, 9, 128), (4, 1, 128), (3, 3, 64), (16, 8, 256)])
+@pytest.mark.parametrize("cap", [0.0, 20.0])
+def test_score_buffers_are_written_again_behind_the_products_that_read_them(ops, heads, kv, dim, cap):
+    """Up to 18 blocks of keys whose probabilities lie over the scores: the formula's values, and the same bits every time."""
+    q, k, v, cu = inputs([2200, 700], heads, kv, dim, torch.bfloat16, seed=dim)
+    cu_t = torch.tensor(cu, dtype=torch.int32, device="cuda")
+    got = ops.prefill_attn(q, k, v, cu_t, dim ** -0.5, softcap=cap)
+    check(got, q, k, v, cu, dim ** -0.5, cap)
+    for _ in range(20):
+        assert torch.equal(ops.prefill_attn(q, k, v, cu_t, dim ** -0.5, softcap=cap), got)
