@@ -523,7 +523,8 @@ int launch_tv(AppendParams p, bool fp8, cudaStream_t stream) {
     static bool attr_done[64] = {};
     int dev = 0;
     cudaGetDevice(&dev);
-    if (smem > 48 * 1024 && dev >= 0 && dev < 64 && !attr_done[dev]) {
+    // (by the first call, whatever it needs: the 48 KB that come by themselves hold the kernel's static arrays as well)
+    if (dev >= 0 && dev < 64 && !attr_done[dev]) {
       const cudaError_t e = cudaFuncSetAttribute(append_fp8_kernel<T, V>, cudaFuncAttributeMaxDynamicSharedMemorySize, 100 * 1024);
       if (e != cudaSuccess) return note_cuda_error(e);
       attr_done[dev] = true;

@@ -2,6 +2,10 @@
 
 Tolerances: the fraction of a turn is rounded once to fp32 and sine and cosine are good to 2 ulp, so both are off by 2^-21 at
 most, and a rotated value by (|x| + |y|) 2^-20 before its one rounding to its type (half of finfo.eps, relative)."""
+import os
+import subprocess
+import sys
+
 import numpy as np
 import pytest
 import torch
@@ -266,3 +270,32 @@ def test_angles_of_far_positions(ops):
         tables = torch.zeros(1, 70000, dtype=torch.int32, device="cuda")
         got = ops.rope_append_kv(x, x, x, cache, cache.clone(), tables, torch.tensor([pos + 1], dtype=torch.int32, device="cuda"), 64)
         check_rotated(got[0].cpu(), x[0].cpu(), pos, 64, 10000.0, 1.0, dtype)
+
+
+def unaligned_first_call(dtype, rotary):
+    """Rows at odd elements, heads of 128: against the 64-bit form (run in a process of its own, as its first append)."""
+    from inference_b200 import ops
+    s, cu = case(dtype, [20, 1], [20, 18], 4, 2, 128, 16, seed=rotary, fp8=True)
+    odd = torch.zeros(21, 8 * 128 + 1, dtype=dtype, device="cuda")
+    odd[:, 1:] = torch.cat([s["q"], s["k"], s["v"]], 1).reshape(21, -1)
+    rows = odd[:, 1:].unflatten(1, (8, 128))
+    s.update(q=rows[:, :4], k=rows[:, 4:6], v=rows[:, 6:])
+    k_out = torch.zeros(21, 2, 128, dtype=dtype, device="cuda")
+    q_got = call(ops, s, rotary, k_out=k_out).cpu()
+    for t, pos, blk, off in places(cu, [20, 18], s["tables"].cpu(), 16, s["k_cache"].shape[0]):
+        check_rotated(q_got[t], s["q"][t].cpu(), pos, rotary, 10000.0, 1.0, dtype)
+        check_rotated(k_out[t].cpu(), s["k"][t].cpu(), pos, rotary, 10000.0, 1.0, dtype)
+        scale = s["v_scales"][blk].cpu()[:, None].double()
+        stored = e4m3(s["v_cache"][blk, off].cpu()) * scale
+        want = s["v"][t].cpu().double()
+        assert bool(((stored - want).abs() <= want.abs() * 2.0 ** -4 + scale * 2.0 ** -10).all())
+
+
+@pytest.mark.parametrize("dtype,rotary", [("bfloat16", 128), ("float16", 128), ("bfloat16", 124), ("float16", 122)])
+def test_unaligned_rows_of_128_in_the_first_call_of_a_process(dtype, rotary):
+    """Shared memory just below 48 KB beside the kernel's own: whether it is granted must not depend on what ran before."""
+    code = f"import test_kv_append_gpu as t, torch; t.unaligned_first_call(torch.{dtype}, {rotary})"
+    here = os.path.dirname(os.path.abspath(__file__))
+    path = os.pathsep.join([here, os.path.dirname(here)])
+    r = subprocess.run([sys.executable, "-c", code], env=dict(os.environ, PYTHONPATH=path), capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
