@@ -150,12 +150,14 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volati
 }
 
 // A row's products of a block -> its scores in base 2: capped, less the distance bias.  ahead: the row's position from the
-// block's first key; behind: no key that counts lies behind the row.
-// tanh: where every score of the warp is within the cap, an odd polynomial of degree 11 (off by 2.4e-7 on [-1, 1], least maximum of
+// block's first key; behind: no key that counts lies behind the row; sees: how many of the block's keys count, the first of them.
+// tanh: where every score of the row is within the cap, an odd polynomial of degree 11 (off by 2.4e-7 on [-1, 1], least maximum of
 // the error) on the FMA units; else 1 - 2 / (1 + e^2x), whose two special functions are the bound of the kernel then (8192
-// tokens, 32 heads of 128: 1640 us against 750).
+// tokens, 32 heads of 128: 1640 us against 750).  A row decides for itself: what it does not see, and what other rows see, has
+// no say in its bits.
 template <int kChunks>
-__device__ __forceinline__ void change_scores(uint32_t (&s)[kChunks][32], const PrefillParams& p, float slope, int ahead, bool behind) {
+__device__ __forceinline__ void change_scores(uint32_t (&s)[kChunks][32], const PrefillParams& p, float slope, int ahead, bool behind,
+                                              int sees) {
   const auto twice = [](float v) { return make_float2(v, v); };
   const float2 f2 = twice(p.scale_log2e);
   if (p.cap_log2e > 0.0f) {
@@ -165,7 +167,16 @@ __device__ __forceinline__ void change_scores(uint32_t (&s)[kChunks][32], const 
 #pragma unroll
       for (int e = 0; e < 32; e += 2) top = max3_abs(top, __uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1]));
     }
-    if (__all_sync(0xFFFFFFFFu, top * fabsf(p.scale_log2e) <= 1.0f)) {   // (NaN is no hindrance: it stays NaN)
+    if (sees < kChunks * 32 && top * fabsf(p.scale_log2e) > 1.0f) {   // it may be one that does not count
+      top = 0.0f;
+#pragma unroll
+      for (int c = 0; c < kChunks; ++c) {
+#pragma unroll
+        for (int e = 0; e < 32; ++e)
+          if (sees > c * 32 + e) top = fmaxf(top, fabsf(__uint_as_float(s[c][e])));
+      }
+    }
+    if (top * fabsf(p.scale_log2e) <= 1.0f) {   // (NaN is no hindrance: it stays NaN)
       const float2 cap2 = twice(p.cap_log2e);
 #pragma unroll
       for (int c = 0; c < kChunks; ++c) {
@@ -193,6 +204,7 @@ __device__ __forceinline__ void change_scores(uint32_t (&s)[kChunks][32], const 
         }
       }
     }
+    __syncwarp();
   } else {
 #pragma unroll
     for (int c = 0; c < kChunks; ++c) {
@@ -544,7 +556,8 @@ prefill_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
           __syncwarp();
           if (lane == 0) mbar_arrive(&s_free[i]);
         }
-        if constexpr (kMod) change_scores<BN / 32>(s, p, slope, pos - j * BN, (j + 1) * BN <= pos_warp + 1 || prefix == 0);
+        if constexpr (kMod)
+          change_scores<BN / 32>(s, p, slope, pos - j * BN, (j + 1) * BN <= pos_warp + 1 || prefix == 0, lim - j * BN);
         if ((j + 1) * BN > lim_warp) {
 #pragma unroll
           for (int c = 0; c < BN / 32; ++c) {
@@ -571,7 +584,8 @@ prefill_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
           if (!ok) break;
           tc_fence_after_sync();
         }
-        // (rows behind the prompt have no say: a prompt's bits do not depend on its neighbours)
+        // (rows behind the prompt have no say: a prompt's bits do not depend on its neighbours; the rows of a warp are one
+        // another's, though, so which of them moved its maximum may show in the others' last bit)
         if (__any_sync(0xFFFFFFFFu, pos < n && (top > m + kRescaleAbove || m == -INFINITY))) {
           const float m_new = fmaxf(m, top);
           const float alpha = m_new == -INFINITY ? 1.0f : ex2(m - m_new);   // (every score so far -inf: no weight, not NaN)

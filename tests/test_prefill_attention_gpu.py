@@ -205,3 +205,37 @@ def test_score_buffers_are_written_again_behind_the_products_that_read_them(ops,
     check(got, q, k, v, cu, dim ** -0.5, cap)
     for _ in range(20):
         assert torch.equal(ops.prefill_attn(q, k, v, cu_t, dim ** -0.5, softcap=cap), got)
+
+
+@pytest.mark.parametrize("heads,kv", [(4, 2), (24, 12), (27, 9)])      # few tiles, pairs of heads, pairs of row tiles
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_capped_scores_that_a_token_does_not_see_do_not_change_its_bits(ops, dim, heads, kv):
+    """Scores within the cap in the prompts that are looked at; far beyond it, infinite or NaN in the others and behind."""
+    lens = [100, 50, 300, 129]
+    q, k, v, cu = (t.clone() if torch.is_tensor(t) else t for t in inputs(lens, heads, kv, dim, torch.float16, seed=3, tail=60))
+    cu_t = torch.tensor(cu, dtype=torch.int32, device="cuda")
+    call = lambda: ops.prefill_attn(q, k, v, cu_t, 0.1, softcap=50.0)
+    clean = call()
+    for t in (q, k):
+        t[cu[1]:cu[2]] *= 100
+        t[cu[4]:] *= 100
+    for value in (None, float("inf"), float("nan")):
+        if value is not None:
+            q[cu[1]:cu[2]] = value
+            k[cu[4]:] = value
+        got = call()
+        for b in (0, 2, 3):
+            assert torch.equal(got[cu[b]:cu[b + 1]], clean[cu[b]:cu[b + 1]]), (value, b)
+    k[cu[2] + 200:cu[3]] *= 100             # keys that earlier tokens do not see (a warp has the rows 192 .. 223)
+    assert torch.equal(call()[cu[2]:cu[2] + 192], clean[cu[2]:cu[2] + 192])
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_rows_within_and_beyond_the_cap_side_by_side(ops, dim):
+    """Rows of one warp of which every third has scores up to some ten times the cap."""
+    q, k, v, cu = inputs([400, 37, 129], 6, 2, dim, torch.bfloat16, seed=dim)
+    q = q.clone()
+    q[::3] *= 32
+    slopes = torch.rand(6, device="cuda") / 8
+    got = ops.prefill_attn(q, k, v, torch.tensor(cu, dtype=torch.int32, device="cuda"), dim ** -0.5, softcap=10.0, alibi_slopes=slopes)
+    check(got, q, k, v, cu, dim ** -0.5, 10.0, slopes)
