@@ -35,14 +35,16 @@ struct AttnWork {
 // What exponents are taken relative to: 0 as long as every score was -inf (their p is 0, not NaN).
 __device__ __forceinline__ float finite_max(float m) { return m == -INFINITY ? 0.0f : m; }
 
-// A capped or biased score in base 2.  x: the product in units of the cap, or in base 2 without one.  tanh(x) =
-// 1 - 2 / (1 + e^2x): off by some 2^-22, which the cap multiplies; at 50 that is 2^-16 of a probability.
+// A capped or biased score in base 2.  x: the product in units of the cap, or in base 2 without one.  tanh(x): up to 1/4 the
+// first terms of its series (off by 62/2835 x^8, 2^-21 relative, at most), beyond it 1 - 2 / (1 + e^2x), off by some 2^-22.  Either
+// way a score is good to 2^-20 of itself, however large the cap (the second form alone: 2^-22 of the cap).
 __device__ __forceinline__ float scored(float x, float cap_log2e, float slope_log2e, int distance) {
   if (cap_log2e > 0.0f) {
     float e, r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(x * 2.885390081777927f));
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
-    x = cap_log2e * fmaf(-2.0f, r, 1.0f);
+    const float z = x * x, series = x * fmaf(z, fmaf(z, fmaf(z, -17.0f / 315.0f, 2.0f / 15.0f), -1.0f / 3.0f), 1.0f);
+    x = cap_log2e * (fabsf(x) <= 0.25f ? series : fmaf(-2.0f, r, 1.0f));
   }
   return fmaf(-slope_log2e, static_cast<float>(distance), x);
 }

@@ -261,3 +261,34 @@ def test_every_step_has_its_blocks_scales(ops, dtype, heads, kv, dim, block):
     close(got, want_of(c, dim ** -0.5), dtype, atol=2e-3)
     for _ in range(20):
         assert torch.equal(call(ops, c, dim ** -0.5), got)
+
+
+@pytest.mark.parametrize("kind", ["fp8", "bf16", "fp16"])
+@pytest.mark.parametrize("form", [0, 1, 2], ids=["auto", "cuda_cores", "tensor_cores"])
+@pytest.mark.parametrize("cap", [3e4, 1e6, 1e9])
+def test_caps_far_above_the_scores(ops, kind, form, cap):
+    """A score's error goes by the score, not by the cap: 2^-20 of it at most, which the default tolerance has room for."""
+    if form and kind == "fp8":
+        pytest.skip("one form only")
+    dtype = torch.float16 if kind == "fp16" else torch.bfloat16
+    ops.set_option("attn_path", form)
+    try:
+        for heads, kv, dim, block, lens in SHAPES[:6]:
+            c = cache_case(heads, kv, dim, block, lens, dtype, seed=heads, fp8=kind == "fp8")
+            close(call(ops, c, dim ** -0.5, softcap=cap), want_of(c, dim ** -0.5, cap), dtype)
+    finally:
+        ops.set_option("attn_path", 0)
+
+
+@pytest.mark.parametrize("kind", ["fp8", "bf16", "fp16"])
+@pytest.mark.parametrize("form", [1, 2], ids=["cuda_cores", "tensor_cores"])
+def test_scores_around_the_cap_of_every_size(ops, kind, form):
+    """Caps from a hundredth of the scores to a hundred times them: every part of the curve."""
+    dtype = torch.float16 if kind == "fp16" else torch.bfloat16
+    ops.set_option("attn_path", form)
+    try:
+        for cap in (0.05, 0.7, 3.0, 9.0, 40.0, 500.0):
+            c = cache_case(8, 2, 128, 16, [40, 700, 3], dtype, seed=int(cap * 100), fp8=kind == "fp8")
+            close(call(ops, c, 0.1, softcap=cap), want_of(c, 0.1, cap), dtype)
+    finally:
+        ops.set_option("attn_path", 0)
