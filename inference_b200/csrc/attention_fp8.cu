@@ -282,11 +282,12 @@ paged_attn_fp8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
     q_scale = p.scale_log2e;
     if constexpr (std::is_same<T, __nv_bfloat16>::value) {
       // bf16 -> fp16 through a power of two that takes the row's maximum to 2^14 .. 2^15: every element down to 2^-28 of
-      // it keeps its eight bits, smaller ones an absolute step of 2^-39 of it
+      // it keeps its eight bits, smaller ones an absolute step of 2^-39 of it.  The power and its inverse are normal numbers for
+      // every finite maximum; one below 2^-112 gets to 2^126 times itself, 1 at least if it is a normal number.
       mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 1));
       mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 2));
       int up = 127 + 14 - static_cast<int>(__float_as_uint(mx) >> 23);
-      up = mx > 0.0f && mx < INFINITY ? max(-100, min(100, up)) : 0;   // (zeros, or an infinity: as they are)
+      up = mx > 0.0f && mx < INFINITY ? min(126, up) : 0;   // (zeros, or an infinity: as they are)
       const float f = __uint_as_float(static_cast<uint32_t>(127 + up) << 23);
       q_scale *= __uint_as_float(static_cast<uint32_t>(127 - up) << 23);
 #pragma unroll

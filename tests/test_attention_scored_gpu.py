@@ -292,3 +292,16 @@ def test_scores_around_the_cap_of_every_size(ops, kind, form):
             close(call(ops, c, 0.1, softcap=cap), want_of(c, 0.1, cap), dtype)
     finally:
         ops.set_option("attn_path", 0)
+
+
+@pytest.mark.parametrize("power", [100, 116, 120, -100, -120])
+def test_query_rows_at_the_ends_of_bf16(ops, power):
+    """A row near 2^power under a scale near its inverse: scores like anybody's."""
+    c = cache_case(4, 2, 128, 16, [64, 200], torch.bfloat16, seed=5)
+    c["q"] = c["q"].clamp(-4, 4)
+    c["q"][:, 1] *= 2.0 ** power
+    scale = 2.0 ** -power * 0.0884
+    want, got = want_of(c, scale), call(ops, c, scale)
+    if power < 0:      # the other rows' scores are without bounds there
+        want, got = want[:, 1:2], got[:, 1:2]
+    close(got, want, torch.bfloat16)
