@@ -239,7 +239,8 @@ INFEROP_API int inferop_rope_neox(void* qkv, const int64_t* positions, int32_t d
  *   q / out [batch, num_heads, head_dim] in dt; k_cache / v_cache [blocks, block_size, num_kv_heads,
  *   head_dim] in dt (16-byte aligned); block_tables int32 [batch, max_blocks_per_seq]; seq_lens int32
  *   [batch] (clamped to max_blocks_per_seq * block_size); out = softmax(q k^T * scale) v per head, an
- *   empty sequence gives zeros.  head_dim in {64, 128, 256} (the reference's list; anything else is
+ *   empty sequence gives zeros.  Other pointers are aligned to their elements (INFEROP_ERR_POINTER
+ *   otherwise).  head_dim in {64, 128, 256} (the reference's list; anything else is
  *   INFEROP_ERR_SHAPE where the reference does nothing), num_heads % num_kv_heads == 0, batch <= 65535.
  * Long sequences are processed as several token ranges whose partial results live in scratch.  fp16 / bf16:
  * 5 MB per stream, or per capture and stream for calls that a CUDA graph captures (given back with the

@@ -711,9 +711,8 @@ static int attn_decode(void* out, const void* q, const void* k_cache, const void
   if (batch > 65535 || static_cast<int64_t>(max_blocks_per_seq) * block_size > 0x7FFFFF00LL) return INFEROP_ERR_LIMIT;
   if (fp8 && static_cast<int64_t>(fp8->num_blocks) * block_size > 0x7FFFFF00LL) return INFEROP_ERR_LIMIT;
   if (!out || !q || !k_cache || !v_cache || !block_tables || !seq_lens) return INFEROP_ERR_POINTER;
-  if ((reinterpret_cast<uintptr_t>(k_cache) & 15u) || (reinterpret_cast<uintptr_t>(v_cache) & 15u)) {
+  if (off(16, {k_cache, v_cache}) || off(4, {block_tables, seq_lens, mod.slopes}) || off(dt == 0 ? 4 : 2, {out, q}))
     return INFEROP_ERR_POINTER;
-  }
   int err;
   DeviceCtx* ctx = current_ctx(&err);
   if (!ctx) return err;
@@ -793,7 +792,6 @@ int inferop_paged_attn_decode_scored(void* out, const void* q, const void* k_cac
                                      int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, int32_t block_size,
                                      int32_t max_blocks_per_seq, float scale, float softcap, const float* alibi_slopes, void* stream) {
   if (!softcap_ok(softcap, scale)) return INFEROP_ERR_SHAPE;
-  if (off(4, {alibi_slopes})) return INFEROP_ERR_POINTER;
   return attn_decode(out, q, k_cache, v_cache, nullptr, block_tables, seq_lens, dt, batch, num_heads, num_kv_heads, head_dim, block_size,
                      max_blocks_per_seq, scale, ScoreMod{softcap, alibi_slopes}, stream);
 }
@@ -804,8 +802,7 @@ int inferop_paged_attn_decode_fp8(void* out, const void* q, const void* k_cache,
                                   int32_t max_blocks_per_seq, float scale, float softcap, const float* alibi_slopes, void* stream) {
   if (block_size % 16 != 0 || num_blocks <= 0 || !softcap_ok(softcap, scale)) return INFEROP_ERR_SHAPE;
   if (dt == 0) return INFEROP_ERR_DTYPE;
-  if (!k_scales || !v_scales || off(4, {k_scales, v_scales, alibi_slopes, block_tables, seq_lens}) || off(2, {q, out}))
-    return INFEROP_ERR_POINTER;
+  if (!k_scales || !v_scales || off(4, {k_scales, v_scales})) return INFEROP_ERR_POINTER;
   const Fp8Cache fp8 = {static_cast<const float*>(k_scales), static_cast<const float*>(v_scales), num_blocks};
   return attn_decode(out, q, k_cache, v_cache, &fp8, block_tables, seq_lens, dt, batch, num_heads, num_kv_heads, head_dim, block_size,
                      max_blocks_per_seq, scale, ScoreMod{softcap, alibi_slopes}, stream);

@@ -117,3 +117,26 @@ def test_native_calls_leave_what_is_not_plain_to_the_general_form():
     assert fast.paged_attn_decode_scored(*[None] * 10) is None
     assert fast.prefill_attn(*[None] * 8) is None
     assert fast.prefill_attn(1, 2) is None
+
+
+def test_decode_lists_queries_and_outputs_off_their_elements():
+    """Every form of the decode attention, plain scores included: refused on the host, not a misaligned address on the device."""
+    no_gpu()
+
+    def call(form, dt=2, out=16, q=16, tables=16, lens=16, slopes=16):
+        head, tail = [out, q, 16, 16], [tables, lens, dt, 1, 8, 4, 128, 16]
+        if form == "plain":
+            return _capi.lib.inferop_paged_attn_decode(*head, *tail, 4, 0.1, None)
+        if form == "scored":
+            return _capi.lib.inferop_paged_attn_decode_scored(*head, *tail, 4, 0.1, 0.0, slopes, None)
+        return _capi.lib.inferop_paged_attn_decode_fp8(*head, 16, 16, *tail, 10, 4, 0.1, 0.0, slopes, None)
+
+    for form in ("plain", "scored", "fp8"):
+        assert call(form) == call(form, out=18, q=22) == _capi.ERR_NO_DEVICE
+        for bad in (dict(tables=18), dict(tables=17), dict(lens=18), dict(lens=19), dict(q=17), dict(out=21)):
+            assert call(form, **bad) == _capi.ERR_POINTER, (form, bad)
+        if form != "plain":
+            assert call(form, slopes=18) == _capi.ERR_POINTER
+        if form != "fp8":
+            assert call(form, dt=0, out=20, q=24) == _capi.ERR_NO_DEVICE
+            assert call(form, dt=0, q=18) == call(form, dt=0, out=18) == _capi.ERR_POINTER
