@@ -255,8 +255,8 @@ INFEROP_API int inferop_paged_attn_decode(void* out, const void* q, const void* 
 
 /* Paged attention decode whose scores s = scale q.k are changed before the softmax: softcap tanh(s / softcap) where
  * softcap > 0, then minus alibi_slopes[head] (seq_len - 1 - t) where there are slopes (fp32 [num_heads], device; NULL:
- * none).  With neither it is inferop_paged_attn_decode, whose contract holds otherwise.  softcap and scale / softcap
- * finite, softcap >= 0.  No counterpart in the reference. */
+ * none).  With neither it is inferop_paged_attn_decode, whose contract holds otherwise.  0 <= softcap <= 1e30 and
+ * scale / softcap finite (INFEROP_ERR_SHAPE otherwise).  No counterpart in the reference. */
 INFEROP_API int inferop_paged_attn_decode_scored(void* out, const void* q, const void* k_cache, const void* v_cache,
                               const int32_t* block_tables, const int32_t* seq_lens, int32_t dt, int32_t batch,
                               int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, int32_t block_size,

@@ -697,7 +697,8 @@ static int kv_append(const KvAppendArgs& a, cudaStream_t s) {
   return launch_kv_append(a, s);
 }
 
-static bool softcap_ok(float cap, float scale) { return cap == 0.0f || (cap > 0.0f && cap < INFINITY && fabsf(scale / cap) < INFINITY); }
+// (above 1e30 the cap to base 2 or a score in units of it would leave fp32's range)
+static bool softcap_ok(float cap, float scale) { return cap == 0.0f || (cap > 0.0f && cap <= 1e30f && fabsf(scale / cap) < INFINITY); }
 
 static int attn_decode(void* out, const void* q, const void* k_cache, const void* v_cache, const Fp8Cache* fp8,
                        const int32_t* block_tables, const int32_t* seq_lens, int32_t dt, int32_t batch, int32_t num_heads,

@@ -140,3 +140,13 @@ def test_decode_lists_queries_and_outputs_off_their_elements():
         if form != "fp8":
             assert call(form, dt=0, out=20, q=24) == _capi.ERR_NO_DEVICE
             assert call(form, dt=0, q=18) == call(form, dt=0, out=18) == _capi.ERR_POINTER
+
+
+def test_caps_whose_units_fp32_cannot_hold():
+    """Above 1e30 the cap to base 2, or a score in units of it, leaves fp32's range (3e38 gave NaN, 1e38 equal weights)."""
+    no_gpu()
+    lib = _capi.lib
+    for cap, want in ((1e30, _capi.ERR_NO_DEVICE), (2e30, _capi.ERR_SHAPE), (1e38, _capi.ERR_SHAPE), (3e38, _capi.ERR_SHAPE)):
+        assert lib.inferop_paged_attn_decode_scored(16, 16, 16, 16, 16, 16, 2, 1, 8, 4, 128, 16, 4, 0.1, cap, None, None) == want
+        assert lib.inferop_paged_attn_decode_fp8(16, 16, 16, 16, 16, 16, 16, 16, 2, 1, 8, 4, 128, 16, 10, 4, 0.1, cap, None, None) == want
+        assert lib.inferop_prefill_attn(16, 1024, 16, 1024, 16, 512, 16, 512, 16, None, 2, 4, 1, 8, 4, 128, 0.1, cap, None, None) == want
