@@ -239,3 +239,26 @@ def test_rows_within_and_beyond_the_cap_side_by_side(ops, dim):
     slopes = torch.rand(6, device="cuda") / 8
     got = ops.prefill_attn(q, k, v, torch.tensor(cu, dtype=torch.int32, device="cuda"), dim ** -0.5, softcap=10.0, alibi_slopes=slopes)
     check(got, q, k, v, cu, dim ** -0.5, 10.0, slopes)
+
+
+@pytest.mark.parametrize("heads,kv", [(27, 9), (16, 16), (9, 3)])
+@pytest.mark.parametrize("cap,bias,prefix", [(0.0, False, False), (20.0, False, False), (0.0, True, True), (20.0, True, True)])
+@pytest.mark.parametrize("lens", [[300, 1, 513, 700, 256, 897], [129, 255, 385, 1024, 640], [1600, 1300, 130, 2100]], ids=["a", "b", "c"])
+def test_pairs_of_row_tiles_of_head_size_64_with_unequal_ends(ops, heads, kv, cap, bias, prefix, lens):
+    """Two tiles of one head whose blocks of keys differ in number, the second one without rows (n % 256 in 1 .. 128) or with some."""
+    q, k, v, cu = inputs(lens, heads, kv, 64, torch.bfloat16, seed=heads + len(lens), lead=1)
+    slopes = torch.exp2(-8.0 * torch.arange(1, heads + 1, device="cuda") / heads) if bias else None
+    pre = torch.tensor([[0, n, 200, 130, n // 2, n + 7][i % 6] for i, n in enumerate(lens)], dtype=torch.int32, device="cuda") if prefix else None
+    got = ops.prefill_attn(q, k, v, torch.tensor(cu, dtype=torch.int32, device="cuda"), 0.125, softcap=cap, alibi_slopes=slopes, prefix_lens=pre)
+    assert ops.device_status()[0] == 0
+    check(got, q, k, v, cu, 0.125, cap, slopes, pre)
+
+
+@pytest.mark.parametrize("heads,kv,dim", [(4, 2, 64), (32, 8, 128), (4, 2, 256)])
+@pytest.mark.parametrize("cap", [3e4, 1e6, 1e9])
+def test_caps_far_above_the_scores(ops, heads, kv, dim, cap):
+    """The polynomial is off by 2^-18 of a score there: 3e-5 of scores up to 16, of which the bound has 5e-5 of the largest value."""
+    q, k, v, cu = inputs([300, 37, 700], heads, kv, dim, torch.float16, seed=dim)
+    q, k = q.clamp(-4, 4), k.clamp(-2, 2)
+    got = ops.prefill_attn(q, k, v, torch.tensor(cu, dtype=torch.int32, device="cuda"), dim ** -0.5 / 2, softcap=cap)
+    check(got, q, k, v, cu, dim ** -0.5 / 2, cap)
