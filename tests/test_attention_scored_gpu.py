@@ -305,3 +305,32 @@ def test_query_rows_at_the_ends_of_bf16(ops, power):
     if power < 0:      # the other rows' scores are without bounds there
         want, got = want[:, 1:2], got[:, 1:2]
     close(got, want, torch.bfloat16)
+
+
+@pytest.mark.parametrize("cap,bias", [(50.0, False), (2000.0, False), (0.0, True), (2000.0, True)])
+def test_fp32_caches_to_fp32s_own_bound(ops, cap, bias):
+    """Short sequences whose weights are of one size, so that a score's error shows.  Bound: a score's sum of 64 products of
+    fp32 in a tree of at most 16 steps, 2^-20 of the products' magnitude; tanhf 2^-22, the bias 2^-23 and the exponential 2^-22
+    of theirs; a weight twice that, times the spread of the values; sums and the output's rounding 8 x 2^-24 of the largest value."""
+    lens = [2, 3, 5, 9, 17, 31]
+    c = cache_case(4, 2, 64, 16, lens, torch.float32, seed=2, fp8=False)
+    scale = 0.03
+    slopes = torch.tensor([0.5, 0.01, 0.1, -0.02]) if bias else None
+    kw = dict(softcap=cap, **(dict(slopes=slopes) if bias else {}))
+    got, want = call(ops, c, scale, **kw).cpu().double(), want_of(c, scale, cap, slopes).cpu()
+    rough = []
+    for b, n in enumerate(lens):
+        k, v = values(c, "k", b), values(c, "v", b)
+        size = (c["q"][b].double().abs()[:, None] * k.repeat_interleave(2, 1).abs().permute(1, 0, 2)).sum(-1) * scale     # [heads, n]
+        far = torch.arange(n - 1, -1, -1).double()
+        score = 2.0 ** -20 * size + 2.0 ** -22 * size + (slopes.abs()[:, None].double() * far * 2.0 ** -23 if bias else 0.0)
+        top = v.abs().amax(0).repeat_interleave(2, 0)                                                                    # [heads, dim]
+        bound = 2 * (score.amax(1)[:, None] + 2.0 ** -22) * top + 8 * 2.0 ** -24 * top
+        assert bool(((got[b] - want[b]).abs() <= bound).all()), (b, float(((got[b] - want[b]).abs() / bound).max()))
+        if cap:    # what 1 - 2 / (1 + e^2x) in fp32 would give: off by more than the bound somewhere at the larger cap
+            x = (torch.einsum("hd,nhd->hn", c["q"][b].double(), k.repeat_interleave(2, 1)) * scale / cap).float()
+            s = (cap * (1 - 2 / (1 + torch.exp2(x * 2.885390081777927)))).double()
+            s = s - (slopes[:, None].double() * far if bias else 0.0)
+            off = torch.einsum("hn,nhd->hd", torch.softmax(s, -1), v.repeat_interleave(2, 1))
+            rough.append(bool(((off - want[b]).abs() > bound).any()))
+    assert cap != 2000.0 or any(rough)
