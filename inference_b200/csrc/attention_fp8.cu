@@ -14,7 +14,7 @@
 //     are the two halves of an operand, and a thread's four scores belong to the four tokens that it holds of V.
 //
 // Bound by instruction latency with twelve warps on an SM, as many as 168 registers allow: 387 instructions per 16 tokens (590 in
-// the form of attention_mma.cu with rows copied by cp.async), 44 % of the issue slots.  Measured (bf16, 32 heads over 8 KV
+// the form of attention_mma.cu with rows copied by cp.async), 43 % of the issue slots while an SM is active.  Measured (bf16, 32 heads over 8 KV
 // heads of 128, blocks of 16 in random order): 64 x 4096 tokens 120 us = 4.5 TB/s (133 us in that form; 173 us
 // over a bf16 cache), 64 x 1000 43 us, one sequence of 777 10.8 us (15); 16 heads over 8 of 256, 64 x 4096: 220 us = 4.9 TB/s; one
 // sequence of 65536, 8 heads over one of 64: 21 us.  A producer warp for all tiles was slower (250 us: its chain of loads

@@ -16,7 +16,7 @@
 //   * Where there are few tiles, a CTA has one, and its two warpgroups take the even and the odd blocks of keys, each with a
 //     maximum, a denominator and sums of its own; they are added at the end.  A long row's chain is half as long.
 //   * A V block and the next K block are one stage of a ring that TMA fills: one wait and one release per block for the
-//     warp that issues the MMAs, whose own time between two products is the tensor cores' idle time (535 -> 525 us below).
+//     warp that issues the MMAs, whose own time between two products is the tensor cores' idle time (2 % of the call below).
 //     V lies as it is (tokens outside): operand B with N contiguous.
 //   * O is rescaled only where a row's maximum grew by more than 2^8 since the last time (the exponentials stay below
 //     that), which is rare behind the first blocks; the row's thread does it in tensor memory.
@@ -25,10 +25,11 @@
 // P is rounded to the operands' type for the second product: 2^-9 (bf16) or 2^-12 relative per term, of random sign, where
 // the sum is rounded to the same type at the end anyway; row sums are of the unrounded values, in fp32.
 //
-// Bound by the tensor cores and, between a tile's two products, by the chain of its softmax: 8192 tokens, 32 heads over 8 KV
-// heads of 128, bf16, causal: 525 us = 1046 TFLOP/s in long runs (at the power cap, 1.67 GHz; 460 us after a pause).  A pair of
-// blocks (256 rows, 128 keys) takes about 3400 cycles, of which the products are 2048 and the softmax of a tile, which the other
-// tile's products run beside, 1850.  Not faster:
+// Bound by the tensor cores and the special-function units, each busy 56 % of the time, and in long runs by the power cap: 8192
+// tokens, 32 heads over 8 KV heads of 128, bf16, causal: 467 us = 1177 TFLOP/s after a pause, 538 us = 1022 in long runs.  Of a
+// pair of blocks (256 rows, 128 keys) the products are 2048 cycles and the softmax of a tile, which the other tile's products run
+// beside, 1850; capped scores 700 us, 16 heads over 8 of 256 510 to 580.  With P over the scores, behind a wait for the product that
+// reads it: 527 to 533 in long runs, capped 755 to 761.  Not faster (P over the scores, without that wait: 525 in long runs):
 // blocks of 64 keys with two score buffers per tile (products of 64 columns run at half the rate: 640 us), a quarter of the
 // exponentials by polynomials (558), P handed over in halves (546), two threads per row (564), an MMA warp per tile (600).
 #include <cuda_bf16.h>
@@ -153,7 +154,7 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volati
 // block's first key; behind: no key that counts lies behind the row; sees: how many of the block's keys count, the first of them.
 // tanh: where every score of the row is within the cap, an odd polynomial of degree 11 (off by 2.4e-7 on [-1, 1], least maximum of
 // the error) on the FMA units; else 1 - 2 / (1 + e^2x), whose two special functions are the bound of the kernel then (8192
-// tokens, 32 heads of 128: 1640 us against 750).  A row decides for itself: what it does not see, and what other rows see, has
+// tokens, 32 heads of 128: 1000 us against 700).  A row decides for itself: what it does not see, and what other rows see, has
 // no say in its bits.
 template <int kChunks>
 __device__ __forceinline__ void change_scores(uint32_t (&s)[kChunks][32], const PrefillParams& p, float slope, int ahead, bool behind,
@@ -534,8 +535,8 @@ prefill_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
       int done = 0;                                          // blocks so far
       // Changed scores: the tiles take turns at their exponentials, so that one changes scores on the FMA units while the other
       // keeps the special-function units busy (without turns they drift into step: 8192 tokens, 16 heads of 64,
-      // cap and bias 429 us, 398 with turns; plain scores 204 and 214; at head size 128, whose turns the
-      // products of the other tile make, capped 730 and 743).
+      // cap and bias 437 us, 410 with turns; plain scores 200 and 218; at head size 128, where the tiles share a score
+      // buffer, capped 702 and 713).
       constexpr bool kTurns = D == 64 && kPairs && kMod;
       const int both = min(t0.blocks, t1.blocks);            // blocks that both tiles have
       for (int j = kHalves ? i : 0; j < t.blocks; j += kStep, ++done) {
@@ -744,10 +745,12 @@ template <typename T, int D, bool kMod>
 int launch_d(const PrefillArgs& a, const PrefillParams& p, cudaStream_t stream) {
   if constexpr (PCfg<D>::kTiles == 2) {
     // A tile per CTA where the longest chain decides, not the sum of the work: all CTAs at once, or, the longer the prompts, up to
-    // two to three per SM.  Two tiles and one, causal, heads of 128: 512 tokens and 32 heads 15 and 12.4 us, 1000 and 8
-    // 19 and 15.5, 4096 and 3 60 and 39; two CTAs per SM: 4096 and 8 64 and 43, 2000 and 16 35 and 30, 4 x 1200 and 6 25.5 and
-    // 24.8, but 1000 and 32 21.6 and 23, 8 x 400 and 8 14 and 19; more: 8192 and 6 122 and 111, 4096 and 12 66 and 68, 2000
-    // and 24 37 and 46, 8192 and 8 120 and 135.
+    // two to three per SM.  Two tiles and one, causal, heads of 128 (of 64 in brackets): 512 tokens and 32 heads 14.1 and 12.2 us (13.0
+    // and 10.6), 1000 and 8 21.1 and 16.3 (19.4 and 13.8), 4096 and 3 65 and 42 (56 and 35); two CTAs per SM: 4096 and 8 65 and 45
+    // (57 and 38), 2000 and 16 36 and 30 (32 and 25), but 1000 and 32 22.1 and 23.2 (19.8 and 19.2), 4 x 1200 and 8 25 and 33 (23 and
+    // 28), 8 x 400 and 8 13.4 and 19.0 (12.5 and 15.8); more: 8192 and 6 126 and 120 (108 and 99), 4096 and 12 67 and 72 (59 and 59),
+    // 2000 and 24 37 and 48 (33 and 39), 8192 and 8 124 and 145 (107 and 120).  Cap and bias: 4096 and 8 110 and 76 (112 and 71),
+    // 512 and 32 20.1 and 16.9, 4 x 1200 and 8 (40 and 42).  Ragged, 1500 + 300 + 800 and 12: 30 and 26, two tiles are taken.
     const int64_t pieces = (a.tokens + static_cast<int64_t>(a.batch) * (kTile - 1)) / kTile;   // at most
     const int64_t mean = a.tokens / a.batch / kTile;
     const int half_ctas = mean >= 64 ? 6 : mean >= 32 ? 5 : mean >= 9 ? 4 : 2;                 // per SM

@@ -15,13 +15,14 @@
 // E4M3: a scale belongs to a cache block and a KV head, so the unit of work is a block, and all of a call's tokens in it
 // belong to one CTA, a warp per head and kind (K, V).  The rows are staged in shared memory and gone through twice, for the
 // maximum and for the bytes: with the rows or the rotated values in registers instead, half as many warps fit an SM, and
-// 16384 tokens took 105 to 116 us for 92.  Scales are powers of two: a floating format loses nothing by them
+// 16384 tokens, half of the head rotated, took 105 to 116 us for 91.  Scales are powers of two: a floating format loses nothing by them
 // (a scale that fits closer would move the values inside a binade), and when a later token needs a larger one, the
 // tokens already there move to it without another rounding (but for E4M3's subnormals).  The values that are quantised
 // are the rotated ones in fp32.
 //
-// Measured (B200): 16384 tokens of 32 + 2 x 8 heads of 128, bf16, with k_out: 75 us = 5.8 TB/s, into E4M3 caches 85 us = 4.8
-// TB/s; one token each of 8 sequences 3.3 us, of 128 sequences into E4M3 caches 5.5 us (launches in a graph).
+// Measured (B200, launches in a graph): 16384 tokens of 32 + 2 x 8 heads of 128, bf16, with k_out: 76 us = 5.7 TB/s, into E4M3
+// caches 86 us = 4.7 TB/s (half of the head rotated 91 us = 4.4); 8192 tokens in fp32 76 us = 5.7 TB/s; E4M3 blocks of 32, 8192 tokens
+// 59 us; one token each of 8 sequences 3.3 us, of 128 sequences into E4M3 caches 5.6 us.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>

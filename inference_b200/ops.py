@@ -530,7 +530,7 @@ def paged_attn_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
     """q [batch, heads, dim]; k_cache / v_cache [blocks, block_size, kv_heads, dim] (q's dtype); block_tables
     int32 [batch, max_blocks]; seq_lens int32 [batch] -> [batch, heads, dim].
 
-    softcap > 0: scores are softcap * tanh(score / softcap).  alibi_slopes fp32 [heads]: then minus the head's slope times a
+    softcap > 0 (1e30 at most): scores are softcap * tanh(score / softcap).  alibi_slopes fp32 [heads]: then minus the head's slope times a
     token's distance from the last one."""
     scored = softcap != 0.0 or alibi_slopes is not None
     if out is None and stream is None:
@@ -609,7 +609,7 @@ def prefill_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: 
 
     cu_seqlens int32 [batch + 1]: prompt b is rows cu_seqlens[b] .. cu_seqlens[b + 1] - 1; other rows of `out` are left as they
     were.  Causal; prefix_lens int32 [batch]: every token of a prompt sees its first so many.  softcap and alibi_slopes as in
-    paged_attn_decode."""
+    paged_attn_decode.  A value row that is not finite may reach tokens of its own prompt that do not see it."""
     if out is None and stream is None and \
             _made(r := fast.prefill_attn(q, k, v, cu_seqlens, scale, softcap, alibi_slopes, prefix_lens), "prefill_attn"):
         return r
