@@ -478,7 +478,8 @@ prefill_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         ok = warp_wait(&full[stage], phase, abort_flag, p.status, kSiteAMmaFull);
         if (!ok) break;
         tc_fence_after_sync();
-        const auto next_scores = [&](int i) {               // of tile i; read: the scores before in the same buffer
+        // (a pair) those of tile i's next block, once the scores before in the same buffer have been read, block `block` of tile `by`
+        const auto next_scores = [&](int i) {
           if (j + 1 >= tile_blocks[i]) return;
           int by = i, block = j;
           if (kOneBuf && i == 0 && j < tile_blocks[1]) by = 1;
