@@ -167,14 +167,14 @@ __device__ __forceinline__ PairOf pair_of(const AppendParams& p, int i) {
   return {2 * i, 2 * i + 1, false};
 }
 
-// a pair of vectors turned
+// a pair of vectors turned (which product is rounded by itself is spelled out: the same bits whatever the form of the call)
 template <int V>
 __device__ __forceinline__ void turn(const float2 (&cs)[V], float (&x0)[V], float (&x1)[V]) {
 #pragma unroll
   for (int e = 0; e < V; ++e) {
     const float f0 = x0[e], f1 = x1[e];
-    x0[e] = f0 * cs[e].x - f1 * cs[e].y;
-    x1[e] = f1 * cs[e].x + f0 * cs[e].y;
+    x0[e] = __fmaf_rn(f0, cs[e].x, -__fmul_rn(f1, cs[e].y));
+    x1[e] = __fmaf_rn(f0, cs[e].y, __fmul_rn(f1, cs[e].x));
   }
 }
 

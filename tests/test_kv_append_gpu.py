@@ -299,3 +299,28 @@ def test_unaligned_rows_of_128_in_the_first_call_of_a_process(dtype, rotary):
     path = os.pathsep.join([here, os.path.dirname(here)])
     r = subprocess.run([sys.executable, "-c", code], env=dict(os.environ, PYTHONPATH=path), capture_output=True, text=True, timeout=300)
     assert r.returncode == 0, r.stderr[-2000:]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim,block", [(64, 16), (128, 32), (256, 48)])
+def test_alignment_and_the_kind_of_cache_do_not_show_in_the_rotated_rows(ops, dtype, dim, block):
+    """Caches of the operands' type and E4M3 ones, rows on 16-byte addresses and at odd elements: the same rotated bits."""
+    new, lens, heads, kv = [70, 1, 33], [100, 9, 33], 6, 3
+    results = []
+    for fp8 in (False, True):
+        s, _ = case(dtype, new, lens, heads, kv, dim, block, seed=dim, fp8=fp8)
+        for odd in (False, True):
+            t = {n: x.clone() for n, x in s.items()}
+            if odd:
+                wide = torch.zeros(104, (heads + 2 * kv) * dim + 1, dtype=dtype, device="cuda")
+                wide[:, 1:] = torch.cat([s["q"], s["k"], s["v"]], 1).reshape(104, -1)
+                rows = wide[:, 1:].unflatten(1, (heads + 2 * kv, dim))
+                t.update(q=rows[:, :heads], k=rows[:, heads:heads + kv], v=rows[:, heads + kv:])
+            k_out = torch.zeros(104, kv, dim, dtype=dtype, device="cuda")
+            q = call(ops, t, dim, k_out=k_out)
+            results.append((q, k_out))
+            if odd:
+                assert all(torch.equal(t[n], last[n]) for n in t if n.endswith(("cache", "scales")))
+            last = t
+    for q, k_out in results[1:]:
+        assert torch.equal(q, results[0][0]) and torch.equal(k_out, results[0][1])
